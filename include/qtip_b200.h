@@ -410,6 +410,82 @@ int qtip_attn_decode_batch(void *out, const void *q, const void *cache_k, const 
                            int n_kv_heads, int head_dim, int max_positions, int batch, long cache_stride, unsigned *status,
                            void *stream);
 
+/* --------------------------------------------------------------------------------------------
+ * Batched decoding over a key/value cache in 8 bits, in blocks of tokens.  A pool holds n_blocks blocks of `block` tokens (16, 32, 64 or 128)
+ * for each layer; `tables` (n_seqs, max_blocks) names the pool's block of each sequence's complete blocks.  Per block and key/value head
+ * there is one scale for K and one for V.  A block is written once, when its last token arrives; until then its tokens stay in fp16 in the
+ * sequence's tail (row length % block onwards is free).  So a value is rounded to 8 bits once, the result does not depend on the pieces
+ * in which tokens were appended, and sequences may share complete blocks by naming the same ones.
+ *   data    (n_blocks, n_kv_heads, block/16, 2, 16*head_dim) bytes   units of 16 tokens: K, then V
+ *           K of a unit: (group of 8 tokens, half of 64 dims, token, dim);  V: token = 8h + 2c + e, dim = g*(head_dim/8) + 4n + j, in the
+ *           order (n, g, c, j, h, e)
+ *   scales  (n_blocks, n_kv_heads, 4) fp32    scale of K, scale of V, two unused
+ *   tail_k  (n_seqs, n_kv_heads, block, head_dim) fp16, tail_v (n_seqs, n_kv_heads, block/2, head_dim, 2) fp16 (pairs of tokens), any stride
+ *           between sequences
+ * QTIP_KV_INT8: value = (byte - 128) * scale, scale = largest magnitude / 127; QTIP_KV_E4M3: value = e4m3 * scale, scale = largest / 448
+ * (the largest is at least 2^-24).  A block in which some value is not finite has the scale NaN: all its tokens stand for NaN.
+ * head_dim 64 or 128.  All follow stream order for every operand.  `status` (optional) as for the decode loop, and 8: the pool is exhausted,
+ * 16: a table names no block of the pool, 32: a beam's parent outside its group.
+ * ------------------------------------------------------------------------------------------ */
+enum { QTIP_KV_INT8 = 0, QTIP_KV_E4M3 = 1 };
+
+/* Where new tokens go.  Sequence s holds lengths[s] tokens and receives new_tokens[s], whose rows follow one another in the order of the
+ * sequences (n_tokens rows in all).  Writes the table entries of the blocks that become complete: the lowest blocks of the pool that no
+ * sequence's complete blocks name, in the order of sequences and positions (a sequence of length 0 holds none, whatever its table says);
+ * lengths_out (n_seqs), not lengths' or new_tokens' buffer; and the new tokens as runs inside one block: runs (max_runs, 8) int32 = sequence,
+ * first token row, first position, tokens, pool block (-1: stays in the tail; -2: in the tail, written with the sequence's first run), for
+ * that first run the number of this one else -1, 0, 0; n_runs their number; rows of `runs` behind it are left as they were.
+ * A sequence that cannot be served (negative numbers, more than max_blocks complete blocks, rows behind n_tokens: status 1; not enough free blocks: status 8)
+ * keeps its length and gets no run.  max_runs >= n_tokens / block + 2 * n_seqs.  runs 16-byte aligned; n_blocks <= 1600000,
+ * n_tokens <= 2^20, positions below 2^31. */
+int qtip_kv_plan(int *tables, const int *lengths, const int *new_tokens, int *lengths_out, int *runs, int *n_runs, int n_seqs, int max_blocks,
+                 int n_blocks, int block, int n_tokens, int max_runs, unsigned *status, void *stream);
+
+/* Rotary embedding of q (n_tokens, n_heads * head_dim; to q_out, which may be q) and k, and append of k and v, along the runs of qtip_kv_plan.  Angle =
+ * position * inv_freq[i] in 64 bits (inv_freq: head_dim/2 doubles), pairs (i, i + head_dim/2); the rotated k is rounded to fp16 before it is
+ * stored or quantised.  Strides in elements between token rows (q, q_out, k, v) and sequences (tails); multiples of 8, pointers 16-byte aligned. */
+int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const void *q, long q_stride, const void *k, long k_stride, const void *v,
+                              long v_stride, void *data, float *scales, void *tail_k, long tail_k_stride, void *tail_v, long tail_v_stride,
+                              const int *runs, const int *n_runs, int max_runs, const double *inv_freq, int n_tokens, int n_seqs, int n_heads,
+                              int n_kv_heads, int head_dim, int n_blocks, int block, int kind, unsigned *status, void *stream);
+
+/* Single-query attention of each sequence over its lengths[s] cached tokens: out, q (n_seqs, n_heads * head_dim) fp16 with row strides; zeros for a
+ * sequence without tokens.  A negative length or one that the table does not hold counts as 0 (status 1).  workspace:
+ * qtip_attn_paged_workspace_bytes() bytes, no initialisation needed; not shared by calls that may overlap.  Strides multiples of 8 elements,
+ * pointers 16-byte aligned. */
+size_t qtip_attn_paged_workspace_bytes(int n_seqs, int n_heads, int n_kv_heads, int head_dim);
+int qtip_attn_decode_paged(void *out, long out_stride, const void *q, long q_stride, const void *data, const float *scales, const void *tail_k,
+                           long tail_k_stride, const void *tail_v, long tail_v_stride, const int *tables, const int *lengths, int n_seqs,
+                           int n_heads, int n_kv_heads, int head_dim, int max_blocks, int n_blocks, int block, int kind, void *workspace,
+                           size_t workspace_bytes, unsigned *status, void *stream);
+
+/* --------------------------------------------------------------------------------------------
+ * Beam search: groups of `width` (<= 16) beams.
+ * ------------------------------------------------------------------------------------------ */
+
+/* The `width` best continuations of each group: largest prev_scores + (logit - log sum exp of the row's logits), sums in 64 bits with the
+ * logarithm rounded to fp32; equal ones in the order of beams, then larger logit, then lower token.  logits (groups * width, vocab) fp32 or fp16 with a row stride; logits
+ * that are not finite are never taken and do not count; a beam whose score is not finite has no continuation; one whose prev_tokens entry is eos
+ * (eos >= 0) has ended and has one: itself, with token eos and its score.  The best continuation of a beam is written to that beam's own row, the
+ * others to the rows left, in order: with parents from here, qtip_beam_reorder copies only rows of beams that are given up.
+ * tokens (groups, width) int64, parents (in the group) int32, scores fp32; tokens / scores may be prev_tokens / prev_scores.  Rows without a
+ * continuation: themselves, token eos (0 without one), score -inf.  A group without any: status 2. */
+int qtip_beam_select(long long *tokens, int *parents, float *scores, const void *logits, int logits_dtype, long logits_stride, const float *prev_scores,
+                     const long long *prev_tokens, int groups, int width, int vocab, long long eos, unsigned *status, void *stream);
+
+/* Row b of each group of states becomes a copy of the group's row parents[b], in place, for any parents (rows may change places).  A state:
+ * (groups * width) sequences, seq_stride bytes apart, of `outer` pieces, outer_stride bytes apart, of `rows` rows of row_bytes (contiguous).
+ * lengths (groups * width) or NULL: only rows below n / per_row, rounded up, are copied, n = the parent's length, modulo `mod` where mod > 0; rows
+ * behind are left as they were.  Bytes and strides multiples of 4; faster at multiples of 16.  A parent outside the group: the row stays
+ * (status 32).  At most 8 states in a call. */
+typedef struct qtip_beam_state {
+    void *base;
+    long seq_stride, outer_stride;
+    int outer, rows, row_bytes, per_row, mod;
+} qtip_beam_state;
+int qtip_beam_reorder(const qtip_beam_state *states, int n_states, const int *parents, const int *lengths, int groups, int width, unsigned *status,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

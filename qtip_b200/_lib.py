@@ -12,6 +12,7 @@ SO_PATH = os.path.join(_HERE, "libqtip_b200.so")
 OK, ERR_BAD_ARG, ERR_BAD_SHAPE, ERR_WORKSPACE, ERR_CUDA, ERR_ALIGNMENT, ERR_TOO_LARGE = range(7)
 CODE_HYB, CODE_3INST, CODE_1MAD = 0, 1, 2
 F16, F32, F16_FRAGMENTS = 0, 1, 2
+KV_INT8, KV_E4M3 = 0, 1
 
 _vp, _i, _l, _sz, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_size_t, ctypes.c_float
 
@@ -23,6 +24,11 @@ class LinearDesc(ctypes.Structure):
                 ("out_scale", _f), ("in_y", _vp), ("in_y_sign", _vp), ("in_y_scale", _f),
                 ("peer_count", _i), ("peer_y", _vp * 8), ("peer_seq", _vp), ("peer_status", _vp),
                 ("peer_max_polls", ctypes.c_uint), ("signal_count", _i), ("signal_y", _vp * 8), ("signal_seq", _vp)]
+
+
+class BeamState(ctypes.Structure):
+    """qtip_beam_state of include/qtip_b200.h."""
+    _fields_ = [("base", _vp), ("seq_stride", _l), ("outer_stride", _l), ("outer", _i), ("rows", _i), ("row_bytes", _i), ("per_row", _i), ("mod", _i)]
 
 
 # name -> (restype, argtypes); mirrors include/qtip_b200.h
@@ -74,6 +80,13 @@ SIGNATURES = {
     "qtip_sample_top_k_batch": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _i, ctypes.c_ulonglong, _i, _vp, _vp]),
     "qtip_rope_kv_append_batch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _l, _vp, _vp]),
     "qtip_attn_decode_batch": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _l, _vp, _vp]),
+    "qtip_kv_plan": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    "qtip_rope_kv_append_paged": (_i, [_vp, _l, _vp, _l, _vp, _l, _vp, _l, _vp, _vp, _vp, _l, _vp, _l, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i,
+                                       _i, _vp, _vp]),
+    "qtip_attn_paged_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "qtip_attn_decode_paged": (_i, [_vp, _l, _vp, _l, _vp, _vp, _vp, _l, _vp, _l, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _vp]),
+    "qtip_beam_select": (_i, [_vp, _vp, _vp, _vp, _i, _l, _vp, _vp, _i, _i, _i, ctypes.c_longlong, _vp, _vp]),
+    "qtip_beam_reorder": (_i, [ctypes.POINTER(BeamState), _i, _vp, _vp, _i, _i, _vp, _vp]),
     "qtip_attn_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

@@ -1,0 +1,411 @@
+// Beam search: the selection of each group's best continuations, and the reordering of what belongs to a beam (caches, block tables,
+// token logs).  They stand where the decode loop samples (eval/interactive_gen.py:15-40 upstream).
+#include "common.cuh"
+
+namespace qtip {
+namespace {
+
+constexpr int kMaxBeams = 16, kMaxStates = 8;
+
+// ---- selection -------------------------------------------------------------------------------------------------------------------
+// A group's beams w < W with scores c_w and logits x_w: the W largest of c_w + (x_wv - lse_w), lse_w = log sum_v exp x_wv.
+// One cluster per group; its 128 warps share the rows.  A warp reads its slice once: the sum of exponentials with a running maximum in each
+// lane, and the W largest logits, which lie sorted in its lanes (a logit that is not above the last of them costs one comparison).  CTA 0
+// merges the lists of a row, one warp per row, adds scores in 64 bits and takes the W largest of the W * W continuations that are left.
+constexpr int kSelectThreads = 512, kSelectCluster = 8, kSelectWarps = kSelectThreads / 32 * kSelectCluster, kSelectHeld = 32;
+
+struct SelectArgs {
+    long long *tokens;
+    int *parents;
+    float *scores;
+    const void *logits;
+    long stride;
+    const float *prev_scores;
+    const long long *prev_tokens;
+    int width, vocab;
+    long long eos;
+    unsigned *status;
+};
+
+struct SelectSmem {
+    unsigned long long keys[kSelectWarps * kMaxBeams];       // (row, warp of the row, rank)
+    float2 sums[kSelectWarps];                               // (row, warp of the row): maximum, sum of exponentials
+    unsigned long long total[kMaxBeams * kMaxBeams];         // ordered bits of the continuations' scores; 0: none
+    int token[kMaxBeams * kMaxBeams];
+};
+
+// Order of floats (doubles) as unsigned integers; 0 is below every number.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);             // -0 and 0 are equal
+    return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+__device__ __forceinline__ unsigned long long ordered(double x) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(x + 0.0);
+    return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double unordered(unsigned long long u) { return __longlong_as_double((long long)(u ^ ((u >> 63) ? 1ull << 63 : ~0ull))); }
+
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
+    const uint32_t hi = __reduce_max_sync(kFullMask, (uint32_t)(v >> 32));
+    const uint32_t lo = __reduce_max_sync(kFullMask, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (unsigned long long)hi << 32 | lo;
+}
+
+template <typename T> struct Vec;
+template <> struct Vec<float> { using type = float4; static constexpr int n = 4; };
+template <> struct Vec<__half> { using type = uint4; static constexpr int n = 8; };
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+
+// One batch of a lane's logits: x[j] is that of index base + place(j), -inf where there is none.
+template <typename T>
+__device__ __forceinline__ void load_batch(float (&x)[kSelectHeld], const T *row, int base, int end, int lane, bool vectors) {
+    constexpr int N = Vec<T>::n;
+    if (vectors && base + 32 * kSelectHeld <= end) {
+#pragma unroll
+        for (int j = 0; j < kSelectHeld / N; j++) {
+            const typename Vec<T>::type v = __ldcs(reinterpret_cast<const typename Vec<T>::type *>(row + base + (j * 32 + lane) * N));
+            const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int k = 0; k < N; k++) x[j * N + k] = to_f(e[k]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kSelectHeld / N; j++)
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const int i = base + (j * 32 + lane) * N + k;
+                x[j * N + k] = i < end ? to_f(row[i]) : -INFINITY;
+            }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSelectThreads) beam_select_kernel(const SelectArgs a) {
+    constexpr int N = Vec<T>::n;
+    __shared__ SelectSmem S;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.width, g = blockIdx.y;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");      // awaited before the first remote store
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int per = kSelectWarps / W, id = (int)rank * (kSelectThreads / 32) + warp, w = id / per, part = id % per;
+    unsigned long long list = 0;                             // lane i < W: the i-th largest (logit, ~index)
+    float m = -INFINITY, sum = 0.f;
+    if (w < W) {
+        const size_t beam = (size_t)g * W + w;
+        const T *row = static_cast<const T *>(a.logits) + beam * (size_t)a.stride;
+        const bool dead = !isfinite(a.prev_scores[beam]) || (a.eos >= 0 && a.prev_tokens && a.prev_tokens[beam] == a.eos);
+        const bool vectors = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+        const int slice = ((a.vocab + per - 1) / per + 7) & ~7;
+        const long long lo = (long long)part * slice;
+        const int end = (int)min((long long)a.vocab, lo + slice);
+        for (long long at = lo; at < end && !dead; at += 32 * kSelectHeld) {
+            float x[kSelectHeld], top = -INFINITY;
+            load_batch<T>(x, row, (int)at, end, lane, vectors);
+#pragma unroll
+            for (int j = 0; j < kSelectHeld; j++) {
+                if (!isfinite(x[j])) x[j] = -INFINITY;
+                top = fmaxf(top, x[j]);
+            }
+            if (top > m) {
+                sum *= exp2f((m - top) * 1.4426950408889634f);         // (m = -inf: 0 times 0)
+                m = top;
+            }
+            if (m > -INFINITY) {
+#pragma unroll
+                for (int j = 0; j < kSelectHeld; j++) sum += exp2f((x[j] - m) * 1.4426950408889634f);
+            }
+            // the W-th largest of the lanes' largest bounds what can enter the list
+            uint32_t mine = top > -INFINITY ? ordered(top) : 0u, bound = 0u;
+            for (int r = 0; r < W; r++) {
+                bound = __reduce_max_sync(kFullMask, mine);
+                const unsigned who = __ballot_sync(kFullMask, mine == bound);
+                if (lane == __ffs(who) - 1) mine = 0u;
+            }
+            bound = max(bound, (uint32_t)(__shfl_sync(kFullMask, list, W - 1) >> 32));
+            if (!__ballot_sync(kFullMask, top > -INFINITY && ordered(top) >= bound)) continue;
+#pragma unroll 1
+            for (int j = 0; j < kSelectHeld; j++) {
+                float v = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < kSelectHeld; q++) v = q == j ? x[q] : v;
+                const uint32_t idx = (uint32_t)((int)at + ((j / N) * 32 + lane) * N + j % N);
+                const unsigned long long key = v > -INFINITY ? (unsigned long long)ordered(v) << 32 | (0xFFFFFFFFu - idx) : 0ull;
+                bool open = (uint32_t)(key >> 32) >= bound && key != 0ull;
+                for (;;) {
+                    const unsigned long long last = __shfl_sync(kFullMask, list, W - 1);
+                    open = open && key > last;
+                    const unsigned who = __ballot_sync(kFullMask, open);
+                    if (!who) break;
+                    const int src = __ffs(who) - 1;
+                    const unsigned long long k = __shfl_sync(kFullMask, key, src), up = __shfl_up_sync(kFullMask, list, 1);
+                    if (k > list) list = lane == 0 || up > k ? k : up;
+                    if (lane == src) open = false;
+                }
+            }
+        }
+        // the lanes' sums
+        float all = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFullMask, all, o));
+        sum = m > -INFINITY ? sum * exp2f((m - all) * 1.4426950408889634f) : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        m = all;
+    }
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (w < W) {
+        uint32_t to;
+        if (lane < W) {
+            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&S.keys[id * W + lane])));
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(list) : "memory");
+        }
+        if (lane == 0) {
+            asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&S.sums[id])));
+            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(m), "f"(sum) : "memory");
+        }
+    }
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    if (rank != 0) return;
+    if (warp < W) {
+        const size_t beam = (size_t)g * W + warp;
+        const float score = a.prev_scores[beam];
+        const bool active = isfinite(score), ended = a.eos >= 0 && a.prev_tokens && a.prev_tokens[beam] == a.eos;
+        // log of the row's sum: terms of 32 bits, added in 64
+        float mx = -INFINITY;
+        for (int i = lane; i < per; i += 32) mx = fmaxf(mx, S.sums[warp * per + i].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
+        double s = 0.0;
+        for (int i = lane; i < per; i += 32) {
+            const float2 v = S.sums[warp * per + i];
+            if (v.y > 0.f) s += (double)v.y * (double)exp2f((v.x - mx) * 1.4426950408889634f);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+        const double lse = (double)(float)((double)mx + log(s));
+        unsigned long long k[kSelectWarps / 32];
+#pragma unroll
+        for (int e = 0; e < kSelectWarps / 32; e++) {
+            const int i = lane + 32 * e;
+            k[e] = i < per * W ? S.keys[warp * per * W + i] : 0ull;
+        }
+        for (int r = 0; r < W; r++) {
+            unsigned long long best = k[0];
+#pragma unroll
+            for (int e = 1; e < kSelectWarps / 32; e++) best = max(best, k[e]);
+            best = warp_max(best);
+#pragma unroll
+            for (int e = 0; e < kSelectWarps / 32; e++)
+                if (k[e] == best) k[e] = 0ull;
+            if (lane == 0) {
+                unsigned long long total = 0ull;
+                int token = (int)(0xFFFFFFFFu - (uint32_t)best);
+                if (active && ended) {
+                    if (r == 0) total = ordered((double)score);
+                    token = -1;
+                } else if (active && best != 0ull) {
+                    total = ordered((double)score + ((double)unordered((uint32_t)(best >> 32)) - lse));
+                }
+                S.total[warp * W + r] = total;
+                S.token[warp * W + r] = token;
+            }
+        }
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    // the W largest; equal ones in the order of beams, then of ranks
+    unsigned long long t[kMaxBeams * kMaxBeams / 32], mine = 0ull;
+    int at = -1;
+#pragma unroll
+    for (int e = 0; e < kMaxBeams * kMaxBeams / 32; e++) t[e] = lane + 32 * e < W * W ? S.total[lane + 32 * e] : 0ull;
+    for (int r = 0; r < W; r++) {
+        unsigned long long best = t[0];
+#pragma unroll
+        for (int e = 1; e < kMaxBeams * kMaxBeams / 32; e++) best = max(best, t[e]);
+        best = warp_max(best);
+        if (best == 0ull) break;
+        uint32_t where = 0xFFFFFFFFu;
+#pragma unroll
+        for (int e = kMaxBeams * kMaxBeams / 32 - 1; e >= 0; e--)
+            if (t[e] == best) where = lane + 32 * e;
+        where = __reduce_min_sync(kFullMask, where);
+#pragma unroll
+        for (int e = 0; e < kMaxBeams * kMaxBeams / 32; e++)
+            if (lane + 32 * e == (int)where) t[e] = 0ull;
+        if (lane == r) { at = (int)where; mine = best; }
+    }
+    // the best continuation of a parent stays in its row, the others fill the rows left, in order
+    const int parent = at >= 0 ? at / W : -1 - lane;
+    const unsigned same = __match_any_sync(kFullMask, parent);
+    const bool stays = at >= 0 && __ffs(same) - 1 == lane, moves = lane < W && !stays;
+    const unsigned taken = __reduce_or_sync(kFullMask, stays ? 1u << parent : 0u), moving = __ballot_sync(kFullMask, moves);
+    if (lane < W) {
+        const int to = stays ? parent : (int)__fns(~taken, 0, __popc(moving & ((1u << lane) - 1)) + 1);
+        const size_t out = (size_t)g * W + to;
+        const int token = at >= 0 ? S.token[at] : -1;
+        a.tokens[out] = token >= 0 ? token : max(a.eos, 0ll);
+        a.parents[out] = at >= 0 ? parent : to;
+        a.scores[out] = at >= 0 ? (float)unordered(mine) : -INFINITY;
+    }
+    if (lane == 0 && at < 0 && a.status) atomicOr(a.status, 2u);
+}
+
+// ---- reordering ------------------------------------------------------------------------------------------------------------------
+// Row b of a group becomes a copy of row parents[b].  A thread owns a column of the group's rows: it reads every row that is to be copied
+// before it writes any, so that rows may be exchanged in place; rows that stay are not touched.
+struct ReorderState {
+    uint8_t *base;
+    long seq_stride, outer_stride;       // bytes
+    int outer, row_bytes, rows, per_row, mod;
+    int vec;                             // bytes of a thread's column: 16, or 4 where the state is not aligned to 16
+    int first;                           // first CTA of this state
+};
+struct ReorderArgs {
+    ReorderState state[kMaxStates];
+    const int *parents, *lengths;
+    int n_states, width;
+    unsigned *status;
+};
+
+constexpr int kReorderThreads = 256;
+
+template <int W, typename V>
+__device__ __forceinline__ void reorder_column(uint8_t *at, long stride, const int *parent, int width) {
+    V v[W];
+#pragma unroll
+    for (int b = 0; b < W; b++)
+        if (b < width && parent[b] != b) v[b] = *reinterpret_cast<const V *>(at + parent[b] * stride);
+#pragma unroll
+    for (int b = 0; b < W; b++)
+        if (b < width && parent[b] != b) *reinterpret_cast<V *>(at + b * stride) = v[b];
+}
+
+template <int W>
+__global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const ReorderArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int parent[W], used[W];
+    const int g = blockIdx.y;
+    bool bad = false;
+    int k = 0;
+    while (k + 1 < a.n_states && (int)blockIdx.x >= a.state[k + 1].first) k++;
+    const ReorderState &s = a.state[k];
+    int most = 0;
+#pragma unroll
+    for (int b = 0; b < W; b++) {
+        parent[b] = b;
+        used[b] = 0;
+        if (b < a.width) {
+            const int p = a.parents[g * a.width + b];
+            if ((unsigned)p < (unsigned)a.width) parent[b] = p;
+            else bad = true;
+            int n = s.rows;
+            if (a.lengths) {
+                n = max(a.lengths[g * a.width + parent[b]], 0);
+                if (s.mod) n %= s.mod;
+                n = min(n / s.per_row + (n % s.per_row != 0), s.rows);
+            }
+            used[b] = parent[b] == b ? 0 : n;
+            most = max(most, used[b]);
+        }
+    }
+    if (bad && a.status && threadIdx.x == 0) atomicOr(a.status, 32u);
+    const int ctas = (k + 1 < a.n_states ? a.state[k + 1].first : (int)gridDim.x) - s.first, cta = blockIdx.x - s.first;
+    const long per_outer = ((long)most * s.row_bytes + s.vec - 1) / s.vec, total = per_outer * s.outer;
+    uint8_t *base = s.base + (long)g * a.width * s.seq_stride;
+    for (long i = (long)cta * kReorderThreads + threadIdx.x; i < total; i += (long)ctas * kReorderThreads) {
+        const long o = i / per_outer, at = (i - o * per_outer) * s.vec;
+        uint8_t *col = base + o * s.outer_stride + at;
+        // a row whose parent is filled less far than another's is copied up to there only, in words
+        int from[W];
+        bool whole = true;
+#pragma unroll
+        for (int b = 0; b < W; b++) {
+            const long left = (long)used[b] * s.row_bytes - at;
+            from[b] = left > 0 ? parent[b] : b;
+            whole &= left <= 0 || left >= s.vec;
+        }
+        if (s.vec == 16 && whole) reorder_column<W, uint4>(col, s.seq_stride, from, a.width);
+        else {
+            for (int j = 0; j < s.vec; j += 4) {
+#pragma unroll
+                for (int b = 0; b < W; b++) from[b] = (long)used[b] * s.row_bytes - at > j ? parent[b] : b;
+                reorder_column<W, uint32_t>(col + j, s.seq_stride, from, a.width);
+            }
+        }
+    }
+}
+
+}  // namespace
+}  // namespace qtip
+
+using namespace qtip;
+
+extern "C" int qtip_beam_select(long long *tokens, int *parents, float *scores, const void *logits, int logits_dtype, long logits_stride,
+                                const float *prev_scores, const long long *prev_tokens, int groups, int width, int vocab, long long eos, unsigned *status,
+                                void *stream) {
+    if (!tokens || !parents || !scores || !logits || !prev_scores || (logits_dtype != QTIP_F16 && logits_dtype != QTIP_F32) || (eos >= 0 && !prev_tokens))
+        return QTIP_ERR_BAD_ARG;
+    if (groups < 1 || groups > 65535 || width < 1 || width > kMaxBeams || vocab < 1 || vocab > (1 << 30) || logits_stride < vocab) return QTIP_ERR_BAD_SHAPE;
+    const SelectArgs a = {tokens, parents, scores, logits, logits_stride, prev_scores, prev_tokens, width, vocab, eos, status};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kSelectCluster, groups);
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kSelectCluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (logits_dtype == QTIP_F32) QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_select_kernel<float>, a));
+    else QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_select_kernel<__half>, a));
+    return check_launch();
+}
+
+extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, const int *parents, const int *lengths, int groups, int width,
+                                 unsigned *status, void *stream) {
+    if (!states || !parents || n_states < 1 || n_states > kMaxStates) return QTIP_ERR_BAD_ARG;
+    if (groups < 1 || groups > 65535 || width < 1 || width > kMaxBeams) return QTIP_ERR_BAD_SHAPE;
+    ReorderArgs a = {};
+    a.parents = parents;
+    a.lengths = lengths;
+    a.n_states = n_states;
+    a.width = width;
+    a.status = status;
+    int ctas = 0;
+    for (int k = 0; k < n_states; k++) {
+        const qtip_beam_state &s = states[k];
+        if (!s.base) return QTIP_ERR_BAD_ARG;
+        if (s.outer < 1 || s.rows < 1 || s.row_bytes < 4 || s.per_row < 1 || s.mod < 0 || (s.row_bytes & 3) || (s.seq_stride & 3) || (s.outer_stride & 3) ||
+            (long)s.rows * s.row_bytes > s.seq_stride || (s.outer > 1 && ((long)s.rows * s.row_bytes > s.outer_stride || (s.outer - 1) * s.outer_stride + (long)s.rows * s.row_bytes > s.seq_stride)))
+            return QTIP_ERR_BAD_SHAPE;
+        if (!aligned(s.base, 4)) return QTIP_ERR_ALIGNMENT;
+        const bool wide = aligned(s.base, 16) && !(s.seq_stride & 15) && (s.outer == 1 || !(s.outer_stride & 15));
+        a.state[k] = {static_cast<uint8_t *>(s.base), s.seq_stride, s.outer_stride, s.outer, s.row_bytes, s.rows, s.per_row, s.mod, wide ? 16 : 4, ctas};
+        const long units = ((long)s.rows * s.row_bytes + a.state[k].vec - 1) / a.state[k].vec * s.outer;
+        const long want = (units + kReorderThreads - 1) / kReorderThreads, most = (long)sm_count() * 8;
+        ctas += (int)(want < most ? want : most);
+    }
+    if (width == 1) return QTIP_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, groups);
+    cfg.blockDim = dim3(kReorderThreads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (width <= 4) QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel<4>, a));
+    else if (width <= 8) QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel<8>, a));
+    else QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel<16>, a));
+    return check_launch();
+}

@@ -31,7 +31,7 @@ struct AttnArgs {
     const __half *tail_k, *tail_v;
     long tail_k_stride, tail_v_stride;
     const int *tables, *lengths;
-    int n_seqs, n_heads, n_kv, max_blocks, n_blocks, block;
+    int n_seqs, n_heads, n_kv, max_blocks, n_blocks, shift;      // block = 1 << shift
     float scale;                     // log2(e) / sqrt(hd)
     float *part_o;                   // (slot, row, hd): sums of a part, not divided
     float2 *part_ml;                 // (slot, row): maximum (in bits of the exponent), sum of weights
@@ -57,7 +57,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
@@ -75,6 +75,12 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi) {
     }
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -86,12 +92,12 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int s, bool *bad = nullptr) {
     int len = a.lengths[s];
-    if (len < 0 || len / a.block > a.max_blocks) {
+    if (len < 0 || len >> a.shift > a.max_blocks) {
         if (bad) *bad = true;
         len = 0;
     }
     Sequence q;
-    q.full = len / a.block * a.block;
+    q.full = len >> a.shift << a.shift;
     q.tail = len - q.full;
     q.coded = (q.full + kTile - 1) / kTile;
     q.tiles = q.coded + (q.tail + kTile - 1) / kTile;
@@ -112,17 +118,18 @@ struct Walk {
     Sequence q;
 };
 
-template <int HD, int KIND>
+template <int HD, int KIND, bool R16>
 __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnArgs a) {
     constexpr int kUnit = 32 * HD, kTileBytes = 2 * kUnit, NT = HD / 8, HALVES = HD / 64;
+    constexpr int UP = R16 ? 2 : 1, E = 2 * UP, kJoin = 2 * NT + 4;              // rows of a lane; values of a lane in a tile of 8 columns
     extern __shared__ __align__(128) uint8_t attn_smem[];
     uint8_t *ring = attn_smem;                                                            // [warp][stage][kTileBytes]
     float4 *ring_scale = reinterpret_cast<float4 *>(attn_smem + kAttnWarps * kStages * kTileBytes);      // [warp][stage][2]
-    float *join = reinterpret_cast<float *>(ring_scale + kAttnWarps * kStages * 2);       // [2][4*NT + 4][32]
+    float *join = reinterpret_cast<float *>(ring_scale + kAttnWarps * kStages * 2);       // [2][kJoin][32]
     __shared__ uint64_t bars[kAttnWarps][kStages];
     __shared__ long long s_tiles[kAttnWarps], s_seqs[kAttnWarps];
     __shared__ Place s_place[2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, b = a.block;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, sh = a.shift, b = 1 << sh;
     const int pairs = a.n_kv * a.groups;                                                  // of a sequence
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid < kAttnWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bars[0][0] + tid)));
@@ -222,12 +229,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
     int ahead_from = ahead.t;
     ahead.t += warp;
     bool more = true;
-    int id0 = 0, id1 = 0;
+    int id0 = 0, id1 = 0, ahead_h = ahead.i / a.groups;
     auto settle = [&]() {                // to this warp's next 8-bit tile, and its blocks' numbers
         while (more && ahead.t >= ahead.t_coded) {
             ahead_left -= ahead.t_end - ahead_from;
             if (ahead_left <= 0) { more = false; break; }
             next_pair(ahead);
+            ahead_h = ahead.i / a.groups;
             ahead.t = ahead_from = 0;
             ahead.left = ahead_left;
             open(ahead);
@@ -236,15 +244,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
         if (more) {
             const int *row = a.tables + (size_t)ahead.s * a.max_blocks;
             const int tok = ahead.t * kTile;
-            id0 = row[tok / b];
-            if (b < kTile) id1 = tok + 16 < ahead.q.full ? row[tok / b + 1] : id0;
+            id0 = row[tok >> sh];
+            if (b < kTile) id1 = tok + 16 < ahead.q.full ? row[(tok >> sh) + 1] : id0;
         }
     };
     unsigned bad_stages = 0;
     uint8_t *my_ring = ring + warp * kStages * kTileBytes;
     float4 *my_scale = ring_scale + warp * kStages * 2;
     auto issue = [&](int stage) {        // copies the tile that settle() found
-        const int tok = ahead.t * kTile, h = ahead.i / a.groups;
+        const int tok = ahead.t * kTile, h = ahead_h;
         const bool two = b < kTile, second = two && tok + 16 < ahead.q.full;
         const bool ok = (unsigned)id0 < (unsigned)a.n_blocks && (unsigned)(two ? id1 : id0) < (unsigned)a.n_blocks;
         bad_stages = (bad_stages & ~(1u << stage)) | (ok ? 0u : 1u << stage);
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
                 if (a.status) atomicOr(a.status, 16u);
             } else {
                 const size_t at = (size_t)id0 * a.n_kv + h;
-                bulk_copy(to, a.data + (at * (b >> 4) + (tok % b >> 4)) * kUnit, two ? kUnit : kTileBytes, bar);
+                bulk_copy(to, a.data + ((at << (sh - 4)) + ((tok & (b - 1)) >> 4)) * kUnit, two ? kUnit : kTileBytes, bar);
                 bulk_copy(to_scale, a.scales + at, 16, bar);
                 if (second) {
                     const size_t at1 = (size_t)id1 * a.n_kv + h;
@@ -291,7 +299,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
 #pragma unroll
             for (int up = 0; up < 2; up++) {
                 uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                if (g + 8 * up < rows) {
+                if (up < UP && g + 8 * up < rows) {
                     const uint4 *p = reinterpret_cast<const uint4 *>(a.q + (size_t)s * a.q_stride + (head0 + g + 8 * up) * HD + half * 64 + c * 16);
                     v[0] = p[0];
                     v[1] = p[1];
@@ -300,26 +308,26 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
 #pragma unroll
                 for (int k = 0; k < 4; k++) { qa[half * 4 + k][up] = r[2 * k]; qa[half * 4 + k][2 + up] = r[2 * k + 1]; }
             }
-        float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, ref = 0.f;      // sums in units of ref
+        float o[NT][4], m[UP], l[UP], ref = 0.f;      // sums in units of ref
+#pragma unroll
+        for (int up = 0; up < UP; up++) { m[up] = -INFINITY; l[up] = 0.f; }
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 4; e++) o[n][e] = 0.f;
 
-        // scores of a tile in bits -> weights, and the sums so far brought to the new maximum
-        auto weigh = [&](float (&x)[4][4]) {
-            float shift[2];
+        // products of a tile -> weights, with sc: bits of the exponent per unit of a product, and the sums so far brought to the new maximum
+        auto weigh = [&](float (&x)[4][4], float sc0, float sc1) {
+            float shift[UP], fix[UP];
             bool moved = false;
-            float fix[2];
 #pragma unroll
-            for (int up = 0; up < 2; up++) {
-                float mx = m[up];
-#pragma unroll
-                for (int n = 0; n < 4; n++) mx = fmaxf(mx, fmaxf(x[n][2 * up], x[n][2 * up + 1]));
+            for (int up = 0; up < UP; up++) {
+                float mx = fmaxf(fmaxf(fmaxf(x[0][2 * up], x[0][2 * up + 1]), fmaxf(x[1][2 * up], x[1][2 * up + 1])) * sc0,
+                                 fmaxf(fmaxf(x[2][2 * up], x[2][2 * up + 1]), fmaxf(x[3][2 * up], x[3][2 * up + 1])) * sc1);
                 mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 2));
+                mx = fmaxf(m[up], fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 2)));
                 const float at = mx == -INFINITY ? 0.f : mx;
-                fix[up] = exp2f(m[up] - at);
+                fix[up] = ex2(m[up] - at);
                 moved |= mx != m[up];
                 m[up] = mx;
                 shift[up] = kLift - at;
@@ -327,15 +335,31 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
             }
             if (__any_sync(kFullMask, moved)) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) { o[n][0] *= fix[0]; o[n][1] *= fix[0]; o[n][2] *= fix[1]; o[n][3] *= fix[1]; }
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[n][e] *= fix[R16 ? e >> 1 : 0];
             }
 #pragma unroll
             for (int n = 0; n < 4; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[n][e] = exp2f(x[n][e] + shift[e >> 1]);
+                for (int e = 0; e < E; e++) {
+                    x[n][e] = ex2(fmaf(x[n][e], n < 2 ? sc0 : sc1, shift[e >> 1]));
                     l[e >> 1] += x[n][e];
                 }
+        };
+        // weights of 16 tokens, times f, as the first operand.  Up to 8 query heads leave the rows 8 to 15 free: they take what the rounding
+        // of the weights to fp16 leaves over, and their sums are added in the end.
+        auto operand = [&](uint32_t (&p)[4], const float (&x)[4][4], int u, float f) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float y0 = x[2 * u + k][0] * f, y1 = x[2 * u + k][1] * f;
+                p[2 * k] = pack(y0, y1);
+                if constexpr (R16) p[2 * k + 1] = pack(x[2 * u + k][2] * f, x[2 * u + k][3] * f);
+                else {
+                    const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&p[2 * k]));
+                    p[2 * k + 1] = pack(y0 - r.x, y1 - r.y);
+                }
+            }
         };
         // brings the sums to a unit that is not below sv; the factor of weights whose values have the scale sv
         auto unit_factor = [&](float sv) {
@@ -361,32 +385,31 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
                 sc[1] = b < kTile ? *reinterpret_cast<const float2 *>(my_scale + stage * 2 + 1) : sc[0];
                 if (bad_stages >> stage & 1) sc[0] = sc[1] = make_float2(NAN, NAN);
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    if (n >= 2 && lone) continue;
+                for (int half = 0; half < HALVES; half++) {
+                    uint4 v[4];
 #pragma unroll
-                    for (int half = 0; half < HALVES; half++) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(tile + (n >> 1) * kUnit + ((n & 1) * HALVES + half) * 512 + lane * 16);
-                        const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+                    for (int n = 0; n < 4; n++)
+                        v[n] = *reinterpret_cast<const uint4 *>(tile + (n >> 1) * kUnit + ((n & 1) * HALVES + half) * 512 + lane * 16);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int n = 0; n < 4; n++) {
                             uint32_t b0, b1;
-                            widen<KIND>(r[k], b0, b1);
+                            widen<KIND>(k == 0 ? v[n].x : k == 1 ? v[n].y : k == 2 ? v[n].z : v[n].w, b0, b1);
                             mma(x[n], qa[half * 4 + k], b0, b1);
                         }
-                    }
                 }
+                if (lone) {
 #pragma unroll
-                for (int n = 0; n < 4; n++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[n][e] = n >= 2 && lone ? -INFINITY : x[n][e] * (a.scale * sc[n >> 1].x);
-                weigh(x);
+                    for (int e = 0; e < E; e++) x[2][e] = x[3][e] = -INFINITY;
+                }
+                weigh(x, a.scale * sc[0].x, lone ? 1.f : a.scale * sc[1].x);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     if (u == 1 && lone) continue;
                     const float f = unit_factor(sc[u].y);
                     uint32_t p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = pack(x[2 * u + (e >> 1)][2 * (e & 1)] * f, x[2 * u + (e >> 1)][2 * (e & 1) + 1] * f);
+                    operand(p, x, u, f);
 #pragma unroll
                     for (int n = 0; n < NT / 4; n++) {
                         const uint4 v = *reinterpret_cast<const uint4 *>(tile + u * kUnit + 16 * HD + n * 512 + lane * 16);
@@ -424,8 +447,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
 #pragma unroll
                 for (int n = 0; n < 4; n++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[n][e] = n * 8 + 2 * c + (e & 1) < n_tok ? x[n][e] * a.scale : -INFINITY;
-                weigh(x);
+                    for (int e = 0; e < E; e++)
+                        if (n * 8 + 2 * c + (e & 1) >= n_tok) x[n][e] = -INFINITY;
+                weigh(x, a.scale, a.scale);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     if (16 * u >= n_tok) continue;
@@ -449,8 +473,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
                     const float up_by = exp2f((float)-e2);
                     const float f = unit_factor(exp2f((float)e2));
                     uint32_t p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = pack(x[2 * u + (e >> 1)][2 * (e & 1)] * f, x[2 * u + (e >> 1)][2 * (e & 1) + 1] * f);
+                    operand(p, x, u, f);
                     auto scaled = [&](uint32_t r) {
                         const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&r));
                         return pack(y.x * up_by, y.y * up_by);
@@ -466,45 +489,52 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
             }
         }
 
-        // ---- the four warps' sums
+        // ---- the four warps' sums, half of the columns at a time
 #pragma unroll
-        for (int up = 0; up < 2; up++) {
+        for (int up = 0; up < UP; up++) {
             l[up] += __shfl_xor_sync(kFullMask, l[up], 1);
             l[up] += __shfl_xor_sync(kFullMask, l[up], 2);
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[n][e] *= ref;
+            for (int e = 0; e < E; e++) o[n][e] = (R16 ? o[n][e] : o[n][e] + o[n][2 + e]) * ref;
+#pragma unroll
         for (int step = 2; step >= 1; step >>= 1) {
-            float *at = join + (warp & (step - 1)) * ((4 * NT + 4) * 32) + lane;
-            if (warp >= step && warp < 2 * step) {
+            float *at = join + (warp & (step - 1)) * (kJoin * 32) + lane;
+            float fa[UP], fb[UP];
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+            for (int half = 0; half < 2; half++) {
+                if (warp >= step && warp < 2 * step) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) at[(4 * n + e) * 32] = o[n][e];
-                at[4 * NT * 32] = m[0];
-                at[(4 * NT + 1) * 32] = m[1];
-                at[(4 * NT + 2) * 32] = l[0];
-                at[(4 * NT + 3) * 32] = l[1];
-            }
-            __syncthreads();
-            if (warp < step) {
-                float fa[2], fb[2];
+                    for (int n = 0; n < NT / 2; n++)
 #pragma unroll
-                for (int up = 0; up < 2; up++) {
-                    const float mb = at[(4 * NT + up) * 32], mx = fmaxf(m[up], mb), ref_m = mx == -INFINITY ? 0.f : mx;
-                    fa[up] = exp2f(m[up] - ref_m);
-                    fb[up] = exp2f(mb - ref_m);
-                    l[up] = l[up] * fa[up] + at[(4 * NT + 2 + up) * 32] * fb[up];
-                    m[up] = mx;
+                        for (int e = 0; e < E; e++) at[(E * n + e) * 32] = o[half * (NT / 2) + n][e];
+                    if (half == 0) {
+#pragma unroll
+                        for (int up = 0; up < UP; up++) { at[(kJoin - 1 - up) * 32] = m[up]; at[(kJoin - 3 - up) * 32] = l[up]; }
+                    }
                 }
+                __syncthreads();
+                if (warp < step) {
+                    if (half == 0) {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                        for (int up = 0; up < UP; up++) {
+                            const float mb = at[(kJoin - 1 - up) * 32], mx = fmaxf(m[up], mb), ref_m = mx == -INFINITY ? 0.f : mx;
+                            fa[up] = ex2(m[up] - ref_m);
+                            fb[up] = ex2(mb - ref_m);
+                            l[up] = l[up] * fa[up] + at[(kJoin - 3 - up) * 32] * fb[up];
+                            m[up] = mx;
+                        }
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[n][e] = o[n][e] * fa[e >> 1] + at[(4 * n + e) * 32] * fb[e >> 1];
+                    for (int n = 0; n < NT / 2; n++)
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            o[half * (NT / 2) + n][e] = o[half * (NT / 2) + n][e] * fa[e >> 1] + at[(E * n + e) * 32] * fb[e >> 1];
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         if (warp == 0) {
             const bool starts = w.t == 0, whole = starts && w.t_end == w.q.tiles;
@@ -527,7 +557,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
                 a.meta[s * pairs + w.i] = make_int2(slot, whole ? 0 : parts);
             }
 #pragma unroll
-            for (int up = 0; up < 2; up++) {
+            for (int up = 0; up < UP; up++) {
                 const int row = g + 8 * up;
                 if (row >= rows) continue;
                 if (whole) {
@@ -587,7 +617,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
         const int slot = k == 0 ? meta.x : 2 * (meta.x / 2 + k);
         const float2 ml = a.part_ml[slot * a.rows + row];
         const float *from = a.part_o + ((size_t)slot * a.rows + row) * HD + lane * E;
-        const float mx = fmaxf(m, ml.x), at = mx == -INFINITY ? 0.f : mx, fa = exp2f(m - at), fb = exp2f(ml.x - at);
+        const float mx = fmaxf(m, ml.x), at = mx == -INFINITY ? 0.f : mx, fa = ex2(m - at), fb = ex2(ml.x - at);
         m = mx;
         l = l * fa + ml.y * fb;
 #pragma unroll
@@ -602,7 +632,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     if (threadIdx.x < HD) {
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float f = exp2f(s_m[w] - at);
+            const float f = ex2(s_m[w] - at);
             sum += s_l[w] * f;
             v += s_o[w][threadIdx.x] * f;
         }
@@ -654,12 +684,15 @@ extern "C" int qtip_attn_decode_paged(void *out, long out_stride, const void *q,
     uint8_t *w = static_cast<uint8_t *>(workspace);
     const AttnArgs a = {static_cast<__half *>(out), static_cast<const __half *>(q), out_stride, q_stride, static_cast<const uint8_t *>(data),
                         reinterpret_cast<const float4 *>(scales), static_cast<const __half *>(tail_k), static_cast<const __half *>(tail_v), tail_k_stride,
-                        tail_v_stride, tables, lengths, n_seqs, n_heads, n_kv_heads, max_blocks, n_blocks, block,
+                        tail_v_stride, tables, lengths, n_seqs, n_heads, n_kv_heads, max_blocks, n_blocks, block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7,
                         1.4426950408889634f / sqrtf((float)head_dim), reinterpret_cast<float *>(w + ws.o), reinterpret_cast<float2 *>(w + ws.ml),
                         reinterpret_cast<int2 *>(w + ws.meta), ws.groups, ws.rows, status};
-    auto kernel = head_dim == 128 ? (kind == kKvInt8 ? attn_paged_kernel<128, kKvInt8> : attn_paged_kernel<128, kKvE4m3>)
-                                  : (kind == kKvInt8 ? attn_paged_kernel<64, kKvInt8> : attn_paged_kernel<64, kKvE4m3>);
-    const size_t smem = (size_t)kAttnWarps * kStages * (64 * head_dim + 32) + (size_t)2 * (head_dim / 2 + 4) * 32 * sizeof(float);
+    const bool r16 = ws.rows > 8;
+    auto kernel = head_dim == 128 ? (kind == kKvInt8 ? (r16 ? attn_paged_kernel<128, kKvInt8, true> : attn_paged_kernel<128, kKvInt8, false>)
+                                                     : (r16 ? attn_paged_kernel<128, kKvE4m3, true> : attn_paged_kernel<128, kKvE4m3, false>))
+                                  : (kind == kKvInt8 ? (r16 ? attn_paged_kernel<64, kKvInt8, true> : attn_paged_kernel<64, kKvInt8, false>)
+                                                     : (r16 ? attn_paged_kernel<64, kKvE4m3, true> : attn_paged_kernel<64, kKvE4m3, false>));
+    const size_t smem = (size_t)kAttnWarps * kStages * (64 * head_dim + 32) + (size_t)2 * (head_dim / 4 + 4) * 32 * sizeof(float);
     QTIP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ws.ctas);

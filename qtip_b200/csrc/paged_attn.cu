@@ -9,15 +9,22 @@
 // them in the order of the tokens.
 // A warp takes every fourth tile of a range.  One of its lanes keeps kStages copies of tiles in flight (a tile of a block of 32 tokens or
 // more is one piece of memory: K and V of 32 tokens); the lanes read the bytes in the order of the operands of the matrix instruction
-// (16 rows: query heads; 16 in depth: dims, then tokens) and widen them to fp16, which holds every code.
-#include <cuda_fp8.h>
+// (K q^T: 16 tokens by 8 query heads, 16 dims deep; V^T p^T: 16 dims by 8 heads, 16 tokens deep) and widen them to fp16, which holds every code.
+#include <type_traits>
+#include <utility>
 
 #include "paged.cuh"
 
 namespace qtip {
 namespace {
 
-constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kStages = 3, kTile = 32, kSnap = 4, kRowsMax = 16;
+constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kTile = 32, kSnap = 4, kRowsMax = 16;
+#ifndef KW
+#define KW 3
+#define KC 64
+#define KF 60
+#endif
+constexpr int kWaves = KW, kChunk = KC, kFirst = KF;
 constexpr float kLift = 15.f;        // weights are 2^15 times exp(score - maximum): fp16 then reaches down to 2^-39 of the largest
 constexpr unsigned kPolls = 1u << 20;
 constexpr int kStatusWait = 64;
@@ -86,198 +93,214 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-struct Sequence {
-    int full, tail;       // tokens in blocks, in the tail
-    int coded, tiles;     // tiles of 8-bit tokens, all tiles
-};
-__device__ __forceinline__ Sequence sequence(const AttnArgs &a, int s, bool *bad = nullptr) {
-    int len = a.lengths[s];
-    if (len < 0 || len >> a.shift > a.max_blocks) {
-        if (bad) *bad = true;
-        len = 0;
-    }
-    Sequence q;
-    q.full = len >> a.shift << a.shift;
-    q.tail = len - q.full;
-    q.coded = (q.full + kTile - 1) / kTile;
-    q.tiles = q.coded + (q.tail + kTile - 1) / kTile;
-    return q;
+// An 8 x 8 matrix of fp16, a row in four lanes, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 
-// A place in the list of all tiles.
-struct Place {
-    long long at;         // tiles before it
-    int s, i, x;          // sequence, pair of it, tile of the pair
-    int tiles;            // of the pair
-};
+constexpr int kTailTile = 16;      // tokens of a tile of the tail: as many bytes as 32 in 8 bits
 
-// Walks over the pairs of a range.
+// A sequence's tokens in blocks, all of them, and tiles of either.
+struct Sequence {
+    int full, len, coded, tiles;
+};
+__device__ __forceinline__ Sequence sequence(const AttnArgs &a, int len) {
+    Sequence q;
+    q.full = len >> a.shift << a.shift;
+    q.len = len;
+    q.coded = (q.full + kTile - 1) / kTile;
+    q.tiles = q.coded + (len - q.full + kTailTile - 1) / kTailTile;
+    return q;
+}
+__device__ __forceinline__ int length_of(const AttnArgs &a, int s) {
+    const int len = a.lengths[s];
+    return len < 0 || len >> a.shift > a.max_blocks ? 0 : len;
+}
+
+// A walk over the parts of pairs in a range of tiles: sequence, pair of it, the part's tiles t0 .. t1, and the range's tiles from t0 on.
 struct Walk {
-    int s, i, t, t_end, t_coded;      // current tile of this warp, end of the pair's part in the range, and of its 8-bit tiles
-    long long left;                   // tiles of the range from the start of this pair's part
+    int s, i, t0, t1, left;
     Sequence q;
 };
 
-template <int HD, int KIND, bool R16>
-__global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnArgs a) {
-    constexpr int kUnit = 32 * HD, kTileBytes = 2 * kUnit, NT = HD / 8, HALVES = HD / 64;
-    constexpr int UP = R16 ? 2 : 1, E = 2 * UP, kJoin = 2 * NT + 4;              // rows of a lane; values of a lane in a tile of 8 columns
+// NB: groups of 8 query heads.
+template <int HD, int NB>
+struct AttnShape {
+    static constexpr int kUnit = 32 * HD, kTileBytes = 2 * kUnit, MT = HD / 16, HALVES = HD / 64;
+    static constexpr int kCtas = NB == 1 ? 3 : 2, kStages = NB == 1 && HD == 128 ? 2 : 3;      // per SM; copies in flight per warp
+    static constexpr int kJoin = NB * 2 * MT;                                                 // half of a lane's sums
+    static constexpr size_t kSmem = (size_t)kAttnWarps * (kStages * (kTileBytes + 32) + (kJoin * 32 + NB * 16) * sizeof(float));
+};
+
+template <int HD, int KIND, int NB>
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_paged_kernel(const AttnArgs a) {
+    using Shape = AttnShape<HD, NB>;
+    constexpr int kUnit = Shape::kUnit, kTileBytes = Shape::kTileBytes, MT = Shape::MT, HALVES = Shape::HALVES, kStages = Shape::kStages, kJoin = Shape::kJoin;
     extern __shared__ __align__(128) uint8_t attn_smem[];
     uint8_t *ring = attn_smem;                                                            // [warp][stage][kTileBytes]
     float4 *ring_scale = reinterpret_cast<float4 *>(attn_smem + kAttnWarps * kStages * kTileBytes);      // [warp][stage][2]
-    float *join = reinterpret_cast<float *>(ring_scale + kAttnWarps * kStages * 2);       // [2][kJoin][32]
+    float *join = reinterpret_cast<float *>(ring_scale + kAttnWarps * kStages * 2);       // [warp][kJoin][32]
+    float2 *join_ml = reinterpret_cast<float2 *>(join + kAttnWarps * kJoin * 32);         // [warp][head of 8 NB]
     __shared__ uint64_t bars[kAttnWarps][kStages];
-    __shared__ long long s_tiles[kAttnWarps], s_seqs[kAttnWarps];
-    __shared__ Place s_place[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, sh = a.shift, b = 1 << sh;
     const int pairs = a.n_kv * a.groups;                                                  // of a sequence
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (tid < kAttnWarps * kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bars[0][0] + tid)));
+    if (lane < kStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bars[warp][lane])));      // a warp's own
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- this CTA's range of tiles
-    const int per = (a.n_seqs + kAttnThreads - 1) / kAttnThreads, s_lo = min(tid * per, a.n_seqs), s_hi = min(s_lo + per, a.n_seqs);
-    long long mine = 0, filled = 0;
-    bool bad = false;
+    // ---- this CTA's range of tiles; every warp computes it, from a piece of the lengths in each lane
+    const int per = (a.n_seqs + 31) >> 5, s_lo = min(lane * per, a.n_seqs), s_hi = min(s_lo + per, a.n_seqs);
+    int mine = 0, seqs = 0;
     for (int s = s_lo; s < s_hi; s++) {
-        const int tiles = sequence(a, s, &bad).tiles;
+        const int tiles = sequence(a, length_of(a, s)).tiles;
         mine += tiles;
-        filled += tiles > 0;
+        seqs += tiles > 0;
     }
-    if (bad && a.status && blockIdx.x == 0) atomicOr(a.status, 1u);
-    long long upto = mine, seqs = filled;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(kFullMask, upto, o), v = __shfl_up_sync(kFullMask, seqs, o);
-        if (lane >= o) { upto += u; seqs += v; }
+        const int u = __shfl_up_sync(kFullMask, upto, o);
+        if (lane >= o) upto += u;
     }
-    if (lane == 31) { s_tiles[warp] = upto; s_seqs[warp] = seqs; }
-    __syncthreads();
-    long long total = 0;
-    seqs = 0;
+    seqs = __reduce_add_sync(kFullMask, seqs);
+    const int total = __shfl_sync(kFullMask, upto, 31) * pairs;
+    // A range is at least four tiles, one per warp, or a pair.  With more work the chip's first CTAs take equal ranges of kFirst % of it, and as many
+    // CTAs per further wave equal ranges of the rest, as the first ones end: some SMs get at the memory faster than others.
+    const int least = max(total / kAttnWarps, seqs * pairs), room = gridDim.x / kWaves;
+    int ctas = max(min(min(total, least), room), 1), share2 = 0, rest2 = 0, early = ctas, early_tiles = total;
+    if (kWaves > 1 && total >= room * kChunk) {
+        ctas = gridDim.x;
+        early = room;
+        early_tiles = total / 100 * kFirst;
+        share2 = (total - early_tiles) / (ctas - early);
+        rest2 = total - early_tiles - share2 * (ctas - early);
+    }
+    const int share = early_tiles / early, rest = early_tiles - share * early;
+    auto border = [&](int cta) {                       // first tile of a CTA's range, before it is moved to a pair's border
+        return cta <= early ? cta * share + min(cta, rest) : early_tiles + (cta - early) * share2 + min(cta - early, rest2);
+    };
+    auto owner = [&](int tile) {                       // the last CTA whose border is not behind the tile
+        const int base = tile < early_tiles ? 0 : early, n = tile < early_tiles ? share : share2, r = tile < early_tiles ? rest : rest2;
+        if (tile >= early_tiles) tile -= early_tiles;
+        return base + (tile < r * (n + 1) ? tile / (n + 1) : (tile - r) / n);
+    };
+    // sequences without tokens: zeros
+    for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x) {
+        if (length_of(a, s) > 0) continue;
+        if (a.lengths[s] != 0 && a.status && tid == 0) atomicOr(a.status, 1u);
+        for (int i = tid; i < a.n_heads * HD / 8; i += kAttnThreads) reinterpret_cast<uint4 *>(a.out + (size_t)s * a.out_stride)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < pairs; i += kAttnThreads) a.meta[s * pairs + i] = make_int2(0, 0);
+    }
+    if (blockIdx.x >= ctas || total == 0) return;
+    int from = 0, length = 0;
+    Walk w;
 #pragma unroll
-    for (int w = 0; w < kAttnWarps; w++) {
-        if (w < warp) upto += s_tiles[w];
-        total += s_tiles[w];
-        seqs += s_seqs[w];
-    }
-    total *= pairs;
-    // at least four tiles each, one per warp, or one pair
-    const long long want = max(total / kAttnWarps, seqs * pairs), ctas = max(min((long long)gridDim.x, min(want, total)), 1ll);
-    const bool works = blockIdx.x < ctas && total > 0;
-    if (works) {
-        for (int k = 0; k < 2; k++) {
-            long long at = (blockIdx.x + k) * total / ctas;
-            if (at >= total) {
-                if (tid == 0) s_place[k] = {total, a.n_seqs, 0, 0, 0};
-            } else if ((upto - mine) * pairs <= at && at < upto * pairs) {
-                long long before = (upto - mine) * pairs;
-                for (int s = s_lo; s < s_hi; s++) {
-                    const int tiles = sequence(a, s).tiles;
-                    if (at < before + (long long)tiles * pairs) {
-                        int i = (int)((at - before) / tiles), x = (int)((at - before) % tiles);
-                        if (x <= kSnap) { at -= x; x = 0; }
-                        else if (tiles - x <= kSnap) { at += tiles - x; x = 0; i++; }
-                        s_place[k] = {at, s, i, x, tiles};
-                        break;
-                    }
-                    before += (long long)tiles * pairs;
+    for (int k = 0; k < 2; k++) {
+        int at = border(blockIdx.x + k), ps = 0, pi = 0, px = 0, plen = 0;
+        const bool here = (upto - mine) * pairs <= at && at < upto * pairs;
+        if (here) {
+            int before = (upto - mine) * pairs;
+            for (int s = s_lo; s < s_hi; s++) {
+                const int len = length_of(a, s), tiles = sequence(a, len).tiles;
+                if (at < before + tiles * pairs) {
+                    ps = s;
+                    plen = len;
+                    pi = (at - before) / tiles;
+                    px = at - before - pi * tiles;
+                    if (px <= kSnap) { at -= px; px = 0; }
+                    else if (tiles - px <= kSnap) { at += tiles - px; px = 0; pi++; }
+                    break;
                 }
+                before += tiles * pairs;
             }
         }
+        const unsigned who = __ballot_sync(kFullMask, here);      // none for the end of all tiles
+        const int src = who ? __ffs(who) - 1 : 0;
+        at = __shfl_sync(kFullMask, at, src);
+        if (k == 1) { length = at - from; break; }
+        from = at;
+        w.s = __shfl_sync(kFullMask, ps, src);
+        w.i = __shfl_sync(kFullMask, pi, src);
+        w.t0 = __shfl_sync(kFullMask, px, src);
+        w.q = sequence(a, __shfl_sync(kFullMask, plen, src));
     }
-    __syncthreads();
-    // sequences without tokens: zeros
-    for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x)
-        if (sequence(a, s).tiles == 0) {
-            for (int i = tid; i < a.n_heads * HD / 8; i += kAttnThreads) reinterpret_cast<uint4 *>(a.out + (size_t)s * a.out_stride)[i] = make_uint4(0, 0, 0, 0);
-            for (int i = tid; i < pairs; i += kAttnThreads) a.meta[s * pairs + i] = make_int2(0, 0);
-        }
-    if (!works) return;
-    const Place from = s_place[0], upto_place = s_place[1];
-    const long long length = upto_place.at - from.at;
     if (length <= 0) return;
 
-    auto open = [&](Walk &w) {           // the part of pair (s, i) from tile w.t on, `left` tiles of the range being left; then this warp's first tile
-        w.t_end = (int)min((long long)w.q.tiles, w.t + w.left);
-        w.t_coded = min(w.t_end, w.q.coded);
-    };
-    auto next_pair = [&](Walk &w) {
-        if (++w.i >= pairs || w.q.tiles == 0) {
-            w.i = 0;
-            do {
-                w.s++;
-                w.q = sequence(a, w.s);
-            } while (w.q.tiles == 0);
+    auto next_pair = [&](Walk &y) {
+        y.t0 = 0;
+        if (++y.i >= pairs) {
+            y.i = 0;
+            do y.q = sequence(a, length_of(a, ++y.s));
+            while (y.q.tiles == 0);
         }
     };
-    auto begin = [&](Walk &w) {
-        w.s = from.s;
-        w.i = from.i;
-        w.t = from.x;
-        w.left = length;
-        w.q = sequence(a, w.s);
-        if (w.i >= pairs) { w.i = pairs - 1; next_pair(w); }
-        open(w);
-    };
+    if (w.i >= pairs) next_pair(w);
+    w.left = length;
+    w.t1 = min(w.q.tiles, w.t0 + w.left);
 
-    // ---- copies of 8-bit tiles, kStages ahead
-    Walk ahead;
-    begin(ahead);
-    long long ahead_left = length;       // tiles of the range from this pair's part on
-    int ahead_from = ahead.t;
-    ahead.t += warp;
+    // ---- copies of this warp's tiles, kStages ahead
+    Walk ahead = w;
+    int ahead_t = w.t0 + warp, ahead_h = w.i / a.groups, id0 = 0, id1 = 0;
     bool more = true;
-    int id0 = 0, id1 = 0, ahead_h = ahead.i / a.groups;
-    auto settle = [&]() {                // to this warp's next 8-bit tile, and its blocks' numbers
-        while (more && ahead.t >= ahead.t_coded) {
-            ahead_left -= ahead.t_end - ahead_from;
-            if (ahead_left <= 0) { more = false; break; }
+    auto settle = [&]() {                // to this warp's next tile, and its blocks' numbers
+        while (more && ahead_t >= ahead.t1) {
+            ahead.left -= ahead.t1 - ahead.t0;
+            if (ahead.left <= 0) { more = false; break; }
             next_pair(ahead);
+            ahead.t1 = min(ahead.q.tiles, ahead.left);
+            ahead_t = warp;
             ahead_h = ahead.i / a.groups;
-            ahead.t = ahead_from = 0;
-            ahead.left = ahead_left;
-            open(ahead);
-            ahead.t = warp;
         }
-        if (more) {
+        if (more && ahead_t < ahead.q.coded) {
             const int *row = a.tables + (size_t)ahead.s * a.max_blocks;
-            const int tok = ahead.t * kTile;
-            id0 = row[tok >> sh];
-            if (b < kTile) id1 = tok + 16 < ahead.q.full ? row[(tok >> sh) + 1] : id0;
+            const int tok = ahead_t * kTile;
+            id0 = id1 = row[tok >> sh];
+            if (b < kTile && tok + 16 < ahead.q.full) id1 = row[(tok >> sh) + 1];
         }
     };
     unsigned bad_stages = 0;
     uint8_t *my_ring = ring + warp * kStages * kTileBytes;
     float4 *my_scale = ring_scale + warp * kStages * 2;
-    auto issue = [&](int stage) {        // copies the tile that settle() found
-        const int tok = ahead.t * kTile, h = ahead_h;
-        const bool two = b < kTile, second = two && tok + 16 < ahead.q.full;
-        const bool ok = (unsigned)id0 < (unsigned)a.n_blocks && (unsigned)(two ? id1 : id0) < (unsigned)a.n_blocks;
-        bad_stages = (bad_stages & ~(1u << stage)) | (ok ? 0u : 1u << stage);
-        if (lane == 0) {
-            const uint32_t bar = smem_u32(&bars[warp][stage]), to = smem_u32(my_ring + stage * kTileBytes), to_scale = smem_u32(my_scale + stage * 2);
-            const uint32_t bytes = !ok ? 0u : two ? (kUnit + 16u) * (second ? 2u : 1u) : kTileBytes + 16u;
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-            if (!ok) {
-                if (a.status) atomicOr(a.status, 16u);
-            } else {
-                const size_t at = (size_t)id0 * a.n_kv + h;
-                bulk_copy(to, a.data + ((at << (sh - 4)) + ((tok & (b - 1)) >> 4)) * kUnit, two ? kUnit : kTileBytes, bar);
-                bulk_copy(to_scale, a.scales + at, 16, bar);
-                if (second) {
-                    const size_t at1 = (size_t)id1 * a.n_kv + h;
-                    bulk_copy(to + kUnit, a.data + at1 * kUnit, kUnit, bar);
-                    bulk_copy(to_scale + 16, a.scales + at1, 16, bar);
+    auto feed = [&](int stage) {         // copies the tile that settle() found, and goes to the next
+        if (!more) return;
+        const uint32_t bar = smem_u32(&bars[warp][stage]), to = smem_u32(my_ring + stage * kTileBytes), to_scale = smem_u32(my_scale + stage * 2);
+        bad_stages &= ~(1u << stage);
+        if (ahead_t >= ahead.q.coded) {
+            const int t0 = (ahead_t - ahead.q.coded) * kTailTile, n = min(kTailTile, ahead.q.len - ahead.q.full - t0);
+            if (lane == 0) {
+                const size_t at = ((size_t)ahead_h * b + t0) * HD;
+                const uint32_t bytes_k = n * HD * 2, bytes_v = (n + 1) / 2 * HD * 4;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes_k + bytes_v) : "memory");
+                bulk_copy(to, a.tail_k + (size_t)ahead.s * a.tail_k_stride + at, bytes_k, bar);
+                bulk_copy(to + kTileBytes / 2, a.tail_v + (size_t)ahead.s * a.tail_v_stride + at, bytes_v, bar);
+            }
+        } else {
+            const int tok = ahead_t * kTile;
+            const bool two = b < kTile, second = two && tok + 16 < ahead.q.full;
+            const bool ok = (unsigned)id0 < (unsigned)a.n_blocks && (unsigned)id1 < (unsigned)a.n_blocks;
+            if (!ok) bad_stages |= 1u << stage;
+            if (lane == 0) {
+                const uint32_t bytes = !ok ? 0u : two ? (kUnit + 16u) * (second ? 2u : 1u) : kTileBytes + 16u;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+                if (!ok) {
+                    if (a.status) atomicOr(a.status, 16u);
+                } else {
+                    const size_t at = (size_t)id0 * a.n_kv + ahead_h;
+                    bulk_copy(to, a.data + ((at << (sh - 4)) + ((tok & (b - 1)) >> 4)) * kUnit, two ? kUnit : kTileBytes, bar);
+                    bulk_copy(to_scale, a.scales + at, 16, bar);
+                    if (second) {
+                        const size_t at1 = (size_t)id1 * a.n_kv + ahead_h;
+                        bulk_copy(to + kUnit, a.data + at1 * kUnit, kUnit, bar);
+                        bulk_copy(to_scale + 16, a.scales + at1, 16, bar);
+                    }
                 }
             }
         }
-    };
-    auto feed = [&](int stage) {
-        if (!more) return;
-        issue(stage);
-        ahead.t += kAttnWarps;
+        ahead_t += kAttnWarps;
         settle();
     };
     settle();
@@ -285,100 +308,112 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
     for (int k = 0; k < kStages; k++) feed(k);
 
     // ---- the range, a pair's part at a time
-    Walk w;
-    begin(w);
-    int w_from = w.t, stage = 0;
+    int stage = 0;
     uint32_t parity = 0;
     bool waited = true, first = true;
     for (;;) {
         const int s = w.s, h = w.i / a.groups, grp = w.i % a.groups, rep = a.n_heads / a.n_kv, head0 = h * rep + grp * kRowsMax, rows = min(kRowsMax, rep - grp * kRowsMax);
-        // q as the first operand: rows g and g + 8, dims 16c + 4k + (0, 1), (2, 3) of step k
-        uint32_t qa[HALVES * 4][4];
+        // q as the second operand: head 8 nb + g, dims 16c + 4k + (0, 1), (2, 3) of step k
+        uint32_t qb[NB][HALVES * 4][2];
 #pragma unroll
-        for (int half = 0; half < HALVES; half++)
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-            for (int up = 0; up < 2; up++) {
+            for (int half = 0; half < HALVES; half++) {
                 uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                if (up < UP && g + 8 * up < rows) {
-                    const uint4 *p = reinterpret_cast<const uint4 *>(a.q + (size_t)s * a.q_stride + (head0 + g + 8 * up) * HD + half * 64 + c * 16);
+                if (8 * nb + g < rows) {
+                    const uint4 *p = reinterpret_cast<const uint4 *>(a.q + (size_t)s * a.q_stride + (head0 + 8 * nb + g) * HD + half * 64 + c * 16);
                     v[0] = p[0];
                     v[1] = p[1];
                 }
                 const uint32_t r[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-                for (int k = 0; k < 4; k++) { qa[half * 4 + k][up] = r[2 * k]; qa[half * 4 + k][2 + up] = r[2 * k + 1]; }
+                for (int k = 0; k < 4; k++) { qb[nb][half * 4 + k][0] = r[2 * k]; qb[nb][half * 4 + k][1] = r[2 * k + 1]; }
             }
-        float o[NT][4], m[UP], l[UP], ref = 0.f;      // sums in units of ref
+        // sums in units of ref: [i][0], [1]: dim g * HD/8 + 2i of heads 2c, 2c + 1; [2], [3]: the next dim.  m, l: of heads 2c, 2c + 1
+        float o[NB][MT][4], m[NB][2], l[NB][2], ref = 0.f;
 #pragma unroll
-        for (int up = 0; up < UP; up++) { m[up] = -INFINITY; l[up] = 0.f; }
+        for (int nb = 0; nb < NB; nb++) {
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+                for (int e = 0; e < 4; e++) o[nb][i][e] = 0.f;
+        }
 
-        // products of a tile -> weights, with sc: bits of the exponent per unit of a product, and the sums so far brought to the new maximum
-        auto weigh = [&](float (&x)[4][4], float sc0, float sc1) {
-            float shift[UP], fix[UP];
+        // products of a tile (x[u]: tokens 16u + g, + 8) -> weights, with sc: bits of the exponent per unit of a product, and the sums so far
+        // brought to the new maximum
+        auto weigh = [&](float (&x)[NB][2][4], float sc0, float sc1) {
+            float shift[NB][2], fix[NB][2];
             bool moved = false;
 #pragma unroll
-            for (int up = 0; up < UP; up++) {
-                float mx = fmaxf(fmaxf(fmaxf(x[0][2 * up], x[0][2 * up + 1]), fmaxf(x[1][2 * up], x[1][2 * up + 1])) * sc0,
-                                 fmaxf(fmaxf(x[2][2 * up], x[2][2 * up + 1]), fmaxf(x[3][2 * up], x[3][2 * up + 1])) * sc1);
-                mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 1));
-                mx = fmaxf(m[up], fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 2)));
-                const float at = mx == -INFINITY ? 0.f : mx;
-                fix[up] = ex2(m[up] - at);
-                moved |= mx != m[up];
-                m[up] = mx;
-                shift[up] = kLift - at;
-                l[up] *= fix[up];
-            }
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][2 + e]) * sc0, fmaxf(x[nb][1][e], x[nb][1][2 + e]) * sc1);
+                    mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 8));
+                    mx = fmaxf(m[nb][e], fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 16)));
+                    const float at = mx == -INFINITY ? 0.f : mx;
+                    fix[nb][e] = ex2(m[nb][e] - at);
+                    moved |= mx != m[nb][e];
+                    m[nb][e] = mx;
+                    shift[nb][e] = kLift - at;
+                }
             if (__any_sync(kFullMask, moved)) {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int nb = 0; nb < NB; nb++) {
+                    l[nb][0] *= fix[nb][0];
+                    l[nb][1] *= fix[nb][1];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[n][e] *= fix[R16 ? e >> 1 : 0];
-            }
+                    for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    x[n][e] = ex2(fmaf(x[n][e], n < 2 ? sc0 : sc1, shift[e >> 1]));
-                    l[e >> 1] += x[n][e];
-                }
-        };
-        // weights of 16 tokens, times f, as the first operand.  Up to 8 query heads leave the rows 8 to 15 free: they take what the rounding
-        // of the weights to fp16 leaves over, and their sums are added in the end.
-        auto operand = [&](uint32_t (&p)[4], const float (&x)[4][4], int u, float f) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const float y0 = x[2 * u + k][0] * f, y1 = x[2 * u + k][1] * f;
-                p[2 * k] = pack(y0, y1);
-                if constexpr (R16) p[2 * k + 1] = pack(x[2 * u + k][2] * f, x[2 * u + k][3] * f);
-                else {
-                    const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&p[2 * k]));
-                    p[2 * k + 1] = pack(y0 - r.x, y1 - r.y);
+                        for (int e = 0; e < 4; e++) o[nb][i][e] *= fix[nb][e & 1];
                 }
             }
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[nb][u][e] = ex2(fmaf(x[nb][u][e], u ? sc1 : sc0, shift[nb][e & 1]));
+                        l[nb][e & 1] += x[nb][u][e];
+                    }
         };
         // brings the sums to a unit that is not below sv; the factor of weights whose values have the scale sv
         auto unit_factor = [&](float sv) {
             if (sv > ref) {
                 const float f = ref / sv;
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[n][e] *= f;
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[nb][i][e] *= f;
                 ref = sv;
             }
-            return ref > 0.f ? sv / ref : sv;
+            return ref > 0.f ? __fdividef(sv, ref) : sv;
+        };
+        // weights of 16 tokens, times f, as the second operand, in two parts of fp16: the second takes what the rounding of the first leaves.
+        // (With one part the error of the result is 1.4 times that of its own rounding to fp16.)
+        auto operand = [&](uint32_t (&p)[2][2], const float (&x)[4], float f) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float y0 = x[2 * k] * f, y1 = x[2 * k + 1] * f;
+                const uint32_t hi = pack(y0, y1);
+                const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                p[0][k] = transposed(hi);
+                p[1][k] = transposed(pack(y0 - r.x, y1 - r.y));
+            }
         };
 
-        for (int t = w.t + warp; t < w.t_end; t += kAttnWarps) {
-            float x[4][4] = {};
-            if (t < w.t_coded) {
-                waited &= bar_wait(smem_u32(&bars[warp][stage]), parity);
-                const uint8_t *tile = my_ring + stage * kTileBytes;
+        for (int t = w.t0 + warp; t < w.t1; t += kAttnWarps) {
+            float x[NB][2][4] = {};
+            uint32_t p[NB][2][2];
+            waited &= bar_wait(smem_u32(&bars[warp][stage]), parity);
+            const uint8_t *tile = my_ring + stage * kTileBytes;
+            if (t < w.q.coded) {
                 const bool lone = b < kTile && t * kTile + 16 >= w.q.full;             // 16 tokens only
                 float2 sc[2];
                 sc[0] = *reinterpret_cast<const float2 *>(my_scale + stage * 2);
@@ -393,205 +428,201 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
 #pragma unroll
                     for (int k = 0; k < 4; k++)
 #pragma unroll
-                        for (int n = 0; n < 4; n++) {
-                            uint32_t b0, b1;
-                            widen<KIND>(k == 0 ? v[n].x : k == 1 ? v[n].y : k == 2 ? v[n].z : v[n].w, b0, b1);
-                            mma(x[n], qa[half * 4 + k], b0, b1);
+                        for (int u = 0; u < 2; u++) {
+                            uint32_t ka[4];
+#pragma unroll
+                            for (int n = 0; n < 2; n++) {
+                                const uint4 &y = v[2 * u + n];
+                                widen<KIND>(k == 0 ? y.x : k == 1 ? y.y : k == 2 ? y.z : y.w, ka[n], ka[2 + n]);
+                            }
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++) mma(x[nb][u], ka, qb[nb][half * 4 + k][0], qb[nb][half * 4 + k][1]);
                         }
                 }
                 if (lone) {
 #pragma unroll
-                    for (int e = 0; e < E; e++) x[2][e] = x[3][e] = -INFINITY;
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[nb][1][e] = -INFINITY;
                 }
                 weigh(x, a.scale * sc[0].x, lone ? 1.f : a.scale * sc[1].x);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     if (u == 1 && lone) continue;
                     const float f = unit_factor(sc[u].y);
-                    uint32_t p[4];
-                    operand(p, x, u, f);
 #pragma unroll
-                    for (int n = 0; n < NT / 4; n++) {
+                    for (int nb = 0; nb < NB; nb++) operand(p[nb], x[nb][u], f);
+#pragma unroll
+                    for (int n = 0; n < MT / 2; n++) {
                         const uint4 v = *reinterpret_cast<const uint4 *>(tile + u * kUnit + 16 * HD + n * 512 + lane * 16);
-                        const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+                        uint32_t va[2][4];
+                        widen<KIND>(v.x, va[0][0], va[0][2]);
+                        widen<KIND>(v.y, va[0][1], va[0][3]);
+                        widen<KIND>(v.z, va[1][0], va[1][2]);
+                        widen<KIND>(v.w, va[1][1], va[1][3]);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            uint32_t b0, b1;
-                            widen<KIND>(r[j], b0, b1);
-                            mma(o[4 * n + j], p, b0, b1);
-                        }
+                        for (int part = 0; part < 2; part++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+#pragma unroll
+                                for (int nb = 0; nb < NB; nb++) mma(o[nb][2 * n + j], va[j], p[nb][part][0], p[nb][part][1]);
                     }
                 }
-                __syncwarp();
-                feed(stage);
-                if (++stage == kStages) { stage = 0; parity ^= 1; }
             } else {
-                // tokens in 16 bits, from the tail
-                const int t0 = (t - w.q.coded) * kTile, n_tok = min(kTile, w.q.tail - t0);
-                const __half *tk = a.tail_k + (size_t)s * a.tail_k_stride + ((size_t)h * b + t0) * HD;
-                const __half *tv = a.tail_v + (size_t)s * a.tail_v_stride + ((size_t)h * b + t0) * HD;
+                // up to 16 tokens in 16 bits, from the tail
+                const int n_tok = min(kTailTile, w.q.len - w.q.full - (t - w.q.coded) * kTailTile);
 #pragma unroll
-                for (int n = 0; n < 4; n++)
+                for (int half = 0; half < HALVES; half++) {
+                    uint4 v[2][2];
 #pragma unroll
-                    for (int half = 0; half < HALVES; half++) {
-                        uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                        if (n * 8 + g < n_tok) {
-                            const uint4 *p = reinterpret_cast<const uint4 *>(tk + (n * 8 + g) * HD + half * 64 + c * 16);
-                            v[0] = p[0];
-                            v[1] = p[1];
-                        }
-                        const uint32_t r[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+                    for (int n = 0; n < 2; n++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) mma(x[n], qa[half * 4 + k], r[2 * k], r[2 * k + 1]);
+                        for (int j = 0; j < 2; j++) v[n][j] = *reinterpret_cast<const uint4 *>(tile + (8 * n + g) * (2 * HD) + half * 128 + c * 32 + j * 16);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint4 &y0 = v[0][k >> 1], &y1 = v[1][k >> 1];
+                        const uint32_t ka[4] = {k & 1 ? y0.z : y0.x, k & 1 ? y1.z : y1.x, k & 1 ? y0.w : y0.y, k & 1 ? y1.w : y1.y};
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) mma(x[nb][0], ka, qb[nb][half * 4 + k][0], qb[nb][half * 4 + k][1]);
                     }
+                }
 #pragma unroll
-                for (int n = 0; n < 4; n++)
+                for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                    for (int e = 0; e < E; e++)
-                        if (n * 8 + 2 * c + (e & 1) >= n_tok) x[n][e] = -INFINITY;
-                weigh(x, a.scale, a.scale);
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    if (16 * u >= n_tok) continue;
-                    uint4 v[2][NT / 4];
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int hh = 0; hh < 2; hh++) {
-                        const int tok = 16 * u + 8 * hh + 2 * c;          // and the next one
-#pragma unroll
-                        for (int n = 0; n < NT / 4; n++) {
-                            v[hh][n] = make_uint4(0, 0, 0, 0);
-                            if (tok < n_tok) v[hh][n] = *reinterpret_cast<const uint4 *>(tv + (size_t)tok * HD + (g * NT + 4 * n) * 2);
-                            if (tok + 1 >= n_tok) { v[hh][n].x &= 0xFFFFu; v[hh][n].y &= 0xFFFFu; v[hh][n].z &= 0xFFFFu; v[hh][n].w &= 0xFFFFu; }
-                            top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[hh][n].x & 0x7FFF7FFFu, v[hh][n].y & 0x7FFF7FFFu),
-                                                         __vmaxu2(v[hh][n].z & 0x7FFF7FFFu, v[hh][n].w & 0x7FFF7FFFu)));
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        if (8 * (e >> 1) + g >= n_tok) x[nb][0][e] = -INFINITY;          // (what lies there is no token)
+                        x[nb][1][e] = -INFINITY;
                     }
-                    // a power of two for the scale, so that small values keep their weights' digits: the exponent that covers all of them
-                    top = __reduce_max_sync(kFullMask, max(top & 0xFFFFu, top >> 16));
-                    const int e2 = top >= 0x7C00u ? 0 : max((int)(top >> 10), 1) - 15 - 6;
-                    const float up_by = exp2f((float)-e2);
-                    const float f = unit_factor(exp2f((float)e2));
-                    uint32_t p[4];
-                    operand(p, x, u, f);
-                    auto scaled = [&](uint32_t r) {
-                        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-                        return pack(y.x * up_by, y.y * up_by);
-                    };
+                weigh(x, a.scale, 1.f);
+                uint4 v[2][MT / 2];
+                uint32_t top = 0;
 #pragma unroll
-                    for (int n = 0; n < NT / 4; n++) {
-                        mma(o[4 * n], p, scaled(v[0][n].x), scaled(v[1][n].x));
-                        mma(o[4 * n + 1], p, scaled(v[0][n].y), scaled(v[1][n].y));
-                        mma(o[4 * n + 2], p, scaled(v[0][n].z), scaled(v[1][n].z));
-                        mma(o[4 * n + 3], p, scaled(v[0][n].w), scaled(v[1][n].w));
+                for (int hh = 0; hh < 2; hh++)
+#pragma unroll
+                    for (int n = 0; n < MT / 2; n++) {
+                        // tokens 8hh + 2c and the next one, dims g * HD/8 + 4n ..; zeros where there is no token
+                        const int tok = 8 * hh + 2 * c;
+                        const uint32_t keep = tok + 1 < n_tok ? 0xFFFFFFFFu : tok < n_tok ? 0xFFFFu : 0u;
+                        uint4 y = *reinterpret_cast<const uint4 *>(tile + kTileBytes / 2 + (4 * hh + c) * (4 * HD) + (g * (HD / 8) + 4 * n) * 4);
+                        y.x &= keep; y.y &= keep; y.z &= keep; y.w &= keep;
+                        v[hh][n] = y;
+                        top = __vmaxu2(top, __vmaxu2(__vmaxu2(y.x & 0x7FFF7FFFu, y.y & 0x7FFF7FFFu), __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
                     }
+                // a power of two for the scale, so that small values keep their weights' digits: the exponent that covers all of them
+                top = __reduce_max_sync(kFullMask, max(top & 0xFFFFu, top >> 16));
+                const int e2 = top >= 0x7C00u ? 0 : max((int)(top >> 10), 1) - 15 - 6;
+                const float up_by = exp2f((float)-e2);
+                const float f = unit_factor(exp2f((float)e2));
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) operand(p[nb], x[nb][0], f);
+                auto scaled = [&](uint32_t r) {
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&r));
+                    return pack(y.x * up_by, y.y * up_by);
+                };
+#pragma unroll
+                for (int n = 0; n < MT / 2; n++) {
+                    const uint32_t va[2][4] = {{scaled(v[0][n].x), scaled(v[0][n].y), scaled(v[1][n].x), scaled(v[1][n].y)},
+                                               {scaled(v[0][n].z), scaled(v[0][n].w), scaled(v[1][n].z), scaled(v[1][n].w)}};
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++) mma(o[nb][2 * n + j], va[j], p[nb][part][0], p[nb][part][1]);
                 }
             }
+            __syncwarp();
+            feed(stage);
+            if (++stage == kStages) { stage = 0; parity ^= 1; }
         }
 
-        // ---- the four warps' sums, half of the columns at a time
+        // ---- the four warps' sums, half of the dims at a time
 #pragma unroll
-        for (int up = 0; up < UP; up++) {
-            l[up] += __shfl_xor_sync(kFullMask, l[up], 1);
-            l[up] += __shfl_xor_sync(kFullMask, l[up], 2);
+        for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                l[nb][e] += __shfl_xor_sync(kFullMask, l[nb][e], 4);
+                l[nb][e] += __shfl_xor_sync(kFullMask, l[nb][e], 8);
+                l[nb][e] += __shfl_xor_sync(kFullMask, l[nb][e], 16);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[nb][i][e] *= ref;
         }
+        const bool starts = w.t0 == 0, whole = starts && w.t1 == w.q.tiles;
+        const int slot = 2 * blockIdx.x + (first ? 0 : 1);
+        float fw[NB][2][kAttnWarps], inv[NB][2];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int half = 0; half < 2; half++) {
+            // all warps' values to shared memory, then each warp adds every fourth tile of dims
 #pragma unroll
-            for (int e = 0; e < E; e++) o[n][e] = (R16 ? o[n][e] : o[n][e] + o[n][2 + e]) * ref;
+            for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
-        for (int step = 2; step >= 1; step >>= 1) {
-            float *at = join + (warp & (step - 1)) * (kJoin * 32) + lane;
-            float fa[UP], fb[UP];
+                for (int i = 0; i < MT / 2; i++)
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                if (warp >= step && warp < 2 * step) {
+                    for (int e = 0; e < 4; e++) join[(warp * kJoin + (nb * (MT / 2) + i) * 4 + e) * 32 + lane] = o[nb][half * (MT / 2) + i][e];
+                if (half == 0 && g == 0) {
 #pragma unroll
-                    for (int n = 0; n < NT / 2; n++)
-#pragma unroll
-                        for (int e = 0; e < E; e++) at[(E * n + e) * 32] = o[half * (NT / 2) + n][e];
-                    if (half == 0) {
-#pragma unroll
-                        for (int up = 0; up < UP; up++) { at[(kJoin - 1 - up) * 32] = m[up]; at[(kJoin - 3 - up) * 32] = l[up]; }
-                    }
+                    for (int e = 0; e < 2; e++) join_ml[warp * 8 * NB + 8 * nb + 2 * c + e] = make_float2(m[nb][e], l[nb][e]);
                 }
-                __syncthreads();
-                if (warp < step) {
-                    if (half == 0) {
-#pragma unroll
-                        for (int up = 0; up < UP; up++) {
-                            const float mb = at[(kJoin - 1 - up) * 32], mx = fmaxf(m[up], mb), ref_m = mx == -INFINITY ? 0.f : mx;
-                            fa[up] = ex2(m[up] - ref_m);
-                            fb[up] = ex2(mb - ref_m);
-                            l[up] = l[up] * fa[up] + at[(kJoin - 3 - up) * 32] * fb[up];
-                            m[up] = mx;
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT / 2; n++)
-#pragma unroll
-                        for (int e = 0; e < E; e++)
-                            o[half * (NT / 2) + n][e] = o[half * (NT / 2) + n][e] * fa[e >> 1] + at[(E * n + e) * 32] * fb[e >> 1];
-                }
-                __syncthreads();
             }
+            __syncthreads();
+            if (half == 0) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float2 y[kAttnWarps];
+                        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+                        for (int v = 0; v < kAttnWarps; v++) { y[v] = join_ml[v * 8 * NB + 8 * nb + 2 * c + e]; mx = fmaxf(mx, y[v].x); }
+                        const float at = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+                        for (int v = 0; v < kAttnWarps; v++) { fw[nb][e][v] = ex2(y[v].x - at); sum += y[v].y * fw[nb][e][v]; }
+                        inv[nb][e] = whole ? 1.f / sum : 1.f;
+                        if (!whole && warp == 0 && g == 0 && 8 * nb + 2 * c + e < rows) a.part_ml[slot * a.rows + 8 * nb + 2 * c + e] = make_float2(mx, sum);
+                    }
+            }
+            for (int i = warp; i < MT / 2; i += kAttnWarps) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    float y[4] = {};
+#pragma unroll
+                    for (int v = 0; v < kAttnWarps; v++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) y[e] = fmaf(join[(v * kJoin + (nb * (MT / 2) + i) * 4 + e) * 32 + lane], fw[nb][e & 1][v], y[e]);
+                    const int d = g * (HD / 8) + 2 * (half * (MT / 2) + i);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int row = 8 * nb + 2 * c + e;
+                        if (row >= rows) continue;
+                        if (whole) *reinterpret_cast<uint32_t *>(a.out + (size_t)s * a.out_stride + (head0 + row) * HD + d) = pack(y[e] * inv[nb][e], y[2 + e] * inv[nb][e]);
+                        else *reinterpret_cast<float2 *>(a.part_o + ((size_t)slot * a.rows + row) * HD + d) = make_float2(y[e], y[2 + e]);
+                    }
+                }
+            }
+            __syncthreads();
         }
-        if (warp == 0) {
-            const bool starts = w.t == 0, whole = starts && w.t_end == w.q.tiles;
-            const int slot = 2 * blockIdx.x + (first ? 0 : 1);
-            if (lane == 0 && starts) {
-                // the CTAs from this one to the one that ends the pair
-                int parts = 1;
-                if (!whole) {
-                    const long long end = from.at + (length - w.left) + w.q.tiles;
-                    long long last = (end - 1) * ctas / total;
-                    last = min(last + 1, ctas - 1);
-                    while (last > blockIdx.x) {
-                        // where that CTA's range begins, as above; inside this pair it is at x of its tiles
-                        const long long at = last * total / ctas, x = at - (end - w.q.tiles);
-                        if (at < end && x > kSnap && w.q.tiles - x > kSnap) break;
-                        last--;
-                    }
-                    parts = (int)(last - blockIdx.x) + 1;
+        if (tid == 0 && starts) {
+            // the CTAs from this one to the one that ends the pair
+            int parts = 0;
+            if (!whole) {
+                const int begins = from + (length - w.left), end = begins + w.q.tiles;
+                int last = owner(end - 1);
+                for (; last > (int)blockIdx.x; last--) {
+                    const int x = border(last) - begins;           // its range begins inside this pair
+                    if (x > kSnap && w.q.tiles - x > kSnap) break;
                 }
-                a.meta[s * pairs + w.i] = make_int2(slot, whole ? 0 : parts);
+                parts = last - (int)blockIdx.x + 1;
             }
-#pragma unroll
-            for (int up = 0; up < UP; up++) {
-                const int row = g + 8 * up;
-                if (row >= rows) continue;
-                if (whole) {
-                    const float inv = 1.f / l[up];
-                    __half *to = a.out + (size_t)s * a.out_stride + (head0 + row) * HD;
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-#pragma unroll
-                        for (int n = 0; n < NT; n += 8) {
-                            uint4 v;
-                            v.x = pack(o[n][2 * up + e] * inv, o[n + 1][2 * up + e] * inv);
-                            v.y = pack(o[n + 2][2 * up + e] * inv, o[n + 3][2 * up + e] * inv);
-                            v.z = pack(o[n + 4][2 * up + e] * inv, o[n + 5][2 * up + e] * inv);
-                            v.w = pack(o[n + 6][2 * up + e] * inv, o[n + 7][2 * up + e] * inv);
-                            *reinterpret_cast<uint4 *>(to + (2 * c + e) * NT + n) = v;
-                        }
-                } else {
-                    float *to = a.part_o + ((size_t)slot * a.rows + row) * HD;
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-#pragma unroll
-                        for (int n = 0; n < NT; n += 4)
-                            *reinterpret_cast<float4 *>(to + (2 * c + e) * NT + n) =
-                                make_float4(o[n][2 * up + e], o[n + 1][2 * up + e], o[n + 2][2 * up + e], o[n + 3][2 * up + e]);
-                    if (c == 0) a.part_ml[slot * a.rows + row] = make_float2(m[up], l[up]);
-                }
-            }
+            a.meta[s * pairs + w.i] = make_int2(slot, parts);
         }
         first = false;
-        w.left -= w.t_end - w_from;
+        w.left -= w.t1 - w.t0;
         if (w.left <= 0) break;
         next_pair(w);
-        w.t = w_from = 0;
-        open(w);
+        w.t1 = min(w.q.tiles, w.left);
     }
     if (!waited) {                       // a copy did not arrive in time: report, and leave only when none is in flight
         if (a.status && lane == 0) atomicOr(a.status, (unsigned)kStatusWait);
@@ -602,41 +633,64 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_paged_kernel(const AttnA
     }
 }
 
-// One CTA per query head and sequence: the parts of its pair, a warp every fourth, then the four sums.
+// One CTA per query head and sequence: joins the parts of its pair, a warp every eighth part.  The weights of the parts come first, so that
+// the loads of their sums do not wait for one another.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+
 template <int HD>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
-    __shared__ float s_o[4][HD], s_m[4], s_l[4];
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnArgs a) {
+    constexpr int E = HD / 32;
+    __shared__ float s_o[kJoinWarps][HD], s_w[kJoinThreads], s_red[2][kJoinWarps];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int rep = a.n_heads / a.n_kv, head = blockIdx.x, in = head % rep, pair = (head / rep) * a.groups + in / kRowsMax, row = in % kRowsMax;
     const int2 meta = a.meta[blockIdx.y * a.n_kv * a.groups + pair];
     if (meta.y == 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = HD / 32;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto slot = [&](int k) { return (size_t)(k == 0 ? meta.x : 2 * (meta.x / 2 + k)) * a.rows + row; };
     float m = -INFINITY, l = 0.f, o[E] = {};
-    for (int k = warp; k < meta.y; k += 4) {
-        const int slot = k == 0 ? meta.x : 2 * (meta.x / 2 + k);
-        const float2 ml = a.part_ml[slot * a.rows + row];
-        const float *from = a.part_o + ((size_t)slot * a.rows + row) * HD + lane * E;
-        const float mx = fmaxf(m, ml.x), at = mx == -INFINITY ? 0.f : mx, fa = ex2(m - at), fb = ex2(ml.x - at);
-        m = mx;
-        l = l * fa + ml.y * fb;
+    for (int k0 = 0; k0 < meta.y; k0 += kJoinThreads) {
+        const float2 ml = k0 + tid < meta.y ? a.part_ml[slot(k0 + tid)] : make_float2(-INFINITY, 0.f);
+        float mx = ml.x;
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * fa + from[e] * fb;
+        for (int o2 = 16; o2 > 0; o2 >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o2));
+        __syncthreads();
+        if (lane == 0) s_red[0][warp] = mx;
+        __syncthreads();
+        mx = m;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; w++) mx = fmaxf(mx, s_red[0][w]);
+        const float at = mx == -INFINITY ? 0.f : mx, fix = ex2(m - at), weight = ex2(ml.x - at);
+        m = mx;
+        s_w[tid] = weight;
+        float sum = ml.y * weight;
+#pragma unroll
+        for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o2);
+        if (lane == 0) s_red[1][warp] = sum;
+        __syncthreads();
+        l *= fix;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; w++) l += s_red[1][w];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= fix;
+#pragma unroll 8
+        for (int k = warp; k < min(kJoinThreads, meta.y - k0); k += kJoinWarps) {
+            const float *from = a.part_o + slot(k0 + k) * HD + lane * E;
+            float v[E];
+            if constexpr (E == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(from);
+            else *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(from);
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = fmaf(v[e], s_w[k], o[e]);
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; e++) s_o[warp][lane * E + e] = o[e];
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
     __syncthreads();
-    const float mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), at = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, v = 0.f;
-    if (threadIdx.x < HD) {
+    if (tid < HD) {
+        float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float f = ex2(s_m[w] - at);
-            sum += s_l[w] * f;
-            v += s_o[w][threadIdx.x] * f;
-        }
-        a.out[(size_t)blockIdx.y * a.out_stride + head * HD + threadIdx.x] = __float2half_rn(v / sum);
+        for (int w = 0; w < kJoinWarps; w++) v += s_o[w][tid];
+        a.out[(size_t)blockIdx.y * a.out_stride + head * HD + tid] = __float2half_rn(v / l);
     }
 }
 
@@ -649,7 +703,7 @@ Workspace workspace_of(int n_seqs, int n_heads, int n_kv, int hd) {
     const int rep = n_heads / n_kv;
     w.groups = (rep + kRowsMax - 1) / kRowsMax;
     w.rows = rep < kRowsMax ? rep : kRowsMax;
-    w.ctas = 2 * sm_count();
+    w.ctas = kWaves * sm_count() * (w.rows > 8 ? AttnShape<128, 2>::kCtas : AttnShape<128, 1>::kCtas);
     w.o = 0;
     w.ml = w.o + (size_t)2 * w.ctas * w.rows * hd * sizeof(float);
     w.meta = w.ml + (size_t)2 * w.ctas * w.rows * sizeof(float2);
@@ -676,6 +730,8 @@ extern "C" int qtip_attn_decode_paged(void *out, long out_stride, const void *q,
         return QTIP_ERR_BAD_SHAPE;
     if (((long)max_blocks + 1) * block > 0x7FFFFFFFl) return QTIP_ERR_BAD_SHAPE;
     const Workspace ws = workspace_of(n_seqs, n_heads, n_kv_heads, head_dim);
+    const int most = (int)(((long)max_blocks * block + kTile - 1) / kTile) + block / kTailTile;                // tiles of a pair
+    if ((long)most * n_seqs * n_kv_heads * ws.groups > 0x3FFFFFFFl) return QTIP_ERR_TOO_LARGE;          // tiles are counted in 32 bits
     if (!workspace || workspace_bytes < ws.bytes) return QTIP_ERR_WORKSPACE;
     const void *ptrs[] = {out, q, data, scales, tail_k, tail_v, workspace};
     for (const void *p : ptrs)
@@ -687,12 +743,13 @@ extern "C" int qtip_attn_decode_paged(void *out, long out_stride, const void *q,
                         tail_v_stride, tables, lengths, n_seqs, n_heads, n_kv_heads, max_blocks, n_blocks, block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7,
                         1.4426950408889634f / sqrtf((float)head_dim), reinterpret_cast<float *>(w + ws.o), reinterpret_cast<float2 *>(w + ws.ml),
                         reinterpret_cast<int2 *>(w + ws.meta), ws.groups, ws.rows, status};
-    const bool r16 = ws.rows > 8;
-    auto kernel = head_dim == 128 ? (kind == kKvInt8 ? (r16 ? attn_paged_kernel<128, kKvInt8, true> : attn_paged_kernel<128, kKvInt8, false>)
-                                                     : (r16 ? attn_paged_kernel<128, kKvE4m3, true> : attn_paged_kernel<128, kKvE4m3, false>))
-                                  : (kind == kKvInt8 ? (r16 ? attn_paged_kernel<64, kKvInt8, true> : attn_paged_kernel<64, kKvInt8, false>)
-                                                     : (r16 ? attn_paged_kernel<64, kKvE4m3, true> : attn_paged_kernel<64, kKvE4m3, false>));
-    const size_t smem = (size_t)kAttnWarps * kStages * (64 * head_dim + 32) + (size_t)2 * (head_dim / 4 + 4) * 32 * sizeof(float);
+    auto pick = [&](auto hd, auto nb) {
+        constexpr int HD = decltype(hd)::value, NB = decltype(nb)::value;
+        return std::make_pair(kind == kKvInt8 ? attn_paged_kernel<HD, kKvInt8, NB> : attn_paged_kernel<HD, kKvE4m3, NB>, AttnShape<HD, NB>::kSmem);
+    };
+    using std::integral_constant;
+    const auto [kernel, smem] = head_dim == 128 ? (ws.rows > 8 ? pick(integral_constant<int, 128>(), integral_constant<int, 2>()) : pick(integral_constant<int, 128>(), integral_constant<int, 1>()))
+                                                : (ws.rows > 8 ? pick(integral_constant<int, 64>(), integral_constant<int, 2>()) : pick(integral_constant<int, 64>(), integral_constant<int, 1>()));
     QTIP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ws.ctas);
@@ -706,9 +763,9 @@ extern "C" int qtip_attn_decode_paged(void *out, long out_stride, const void *q,
     cfg.numAttrs = 1;
     QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
     // a pair of at most 2 * kSnap tiles is never cut
-    if (((long)max_blocks * block + kTile - 1) / kTile + (block - 1 + kTile - 1) / kTile > 2 * kSnap) {
+    if (most > 2 * kSnap) {
         cfg.gridDim = dim3(n_heads, n_seqs);
-        cfg.blockDim = dim3(128);
+        cfg.blockDim = dim3(kJoinThreads);
         cfg.dynamicSmemBytes = 0;
         QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, head_dim == 128 ? attn_join_kernel<128> : attn_join_kernel<64>, a));
     }

@@ -255,14 +255,16 @@ __global__ void __launch_bounds__(kSelectThreads) beam_select_kernel(const Selec
 }
 
 // ---- reordering ------------------------------------------------------------------------------------------------------------------
-// Row b of a group becomes a copy of row parents[b].  A thread owns a column of the group's rows: it reads every row that is to be copied
-// before it writes any, so that rows may be exchanged in place; rows that stay are not touched.
+// Row b of a group becomes a copy of row parents[b].  Rows that stay are not touched.  Bound by the bytes of the rows that are copied.
+// A thread owns columns of the group's rows and makes all copies of them in an order in which no row is read after it was written: where no
+// row that is copied from is itself replaced (beam_select's parents), any order, with several loads in flight; else rows that nobody
+// needs any more first, and then what is left, cycles, through a register.
 struct ReorderState {
     uint8_t *base;
     long seq_stride, outer_stride;       // bytes
     int outer, row_bytes, rows, per_row, mod;
-    int vec;                             // bytes of a thread's column: 16, or 4 where the state is not aligned to 16
     int first;                           // first CTA of this state
+    int wide;                            // columns of 16 bytes, else of 4
 };
 struct ReorderArgs {
     ReorderState state[kMaxStates];
@@ -271,73 +273,148 @@ struct ReorderArgs {
     unsigned *status;
 };
 
-constexpr int kReorderThreads = 256;
+constexpr int kReorderThreads = 256, kReorderColumns = 4;
 
-template <int W, typename V>
-__device__ __forceinline__ void reorder_column(uint8_t *at, long stride, const int *parent, int width) {
-    V v[W];
-#pragma unroll
-    for (int b = 0; b < W; b++)
-        if (b < width && parent[b] != b) v[b] = *reinterpret_cast<const V *>(at + parent[b] * stride);
-#pragma unroll
-    for (int b = 0; b < W; b++)
-        if (b < width && parent[b] != b) *reinterpret_cast<V *>(at + b * stride) = v[b];
+struct Moves {
+    int n;                               // steps
+    int ordered;                         // they have to be made one after another
+    int to[2 * kMaxBeams], from[2 * kMaxBeams];      // rows; to -1: into the register, from -1: out of it
+    int bytes[2 * kMaxBeams];            // of a piece, from its start
+};
+
+// One thread; rarely needed.
+__device__ __noinline__ void order_moves(Moves &m, const int *parent, const int *bytes, int width) {
+    unsigned left = 0;
+    for (int b = 0; b < width; b++)
+        if (parent[b] != b) left |= 1u << b;
+    int n = 0;
+    while (left) {
+        int pick = -1;
+        for (int b = 0; b < width && pick < 0; b++) {
+            if (!(left >> b & 1)) continue;
+            bool needed = false;
+            for (int o = 0; o < width; o++) needed |= (left >> o & 1) && parent[o] == b;
+            if (!needed) pick = b;
+        }
+        if (pick >= 0) {
+            m.to[n] = pick; m.from[n] = parent[pick]; m.bytes[n++] = bytes[pick];
+            left &= ~(1u << pick);
+            continue;
+        }
+        // a cycle: its first row is kept, each row takes its parent's, the last the kept one
+        const int start = __ffs(left) - 1;
+        m.to[n] = -1; m.from[n] = start; m.bytes[n++] = 0x7FFFFFFF;
+        for (int b = start;;) {
+            const int p = parent[b];
+            m.to[n] = b; m.from[n] = p == start ? -1 : p; m.bytes[n++] = bytes[b];
+            left &= ~(1u << b);
+            if (p == start) break;
+            b = p;
+        }
+    }
+    m.n = n;
 }
 
-template <int W>
+template <typename V>
+__device__ __forceinline__ void copy_columns(const ReorderState &s, const Moves &m, uint8_t *base, int per_outer, int total, int cta, int ctas) {
+    constexpr int kBytes = sizeof(V), U = kReorderColumns;
+    const int stride = ctas * kReorderThreads;
+    for (int i0 = cta * kReorderThreads + threadIdx.x; i0 < total; i0 += U * stride) {
+        uint8_t *col[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const unsigned i = (unsigned)i0 + (unsigned)u * stride, o = i / (unsigned)per_outer;
+            at[u] = i < (unsigned)total ? (int)((i - o * per_outer) * kBytes) : 0x7FFFFFFF - 16;      // behind every row
+            col[u] = base + (long)o * s.outer_stride + (i - o * per_outer) * kBytes;
+        }
+        if (!m.ordered) {
+            for (int k = 0; k < m.n; k++) {
+                const long to = m.to[k] * s.seq_stride, from = m.from[k] * s.seq_stride;
+                const int bytes = m.bytes[k];
+                V v[U];
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (at[u] + kBytes <= bytes) v[u] = __ldcs(reinterpret_cast<const V *>(col[u] + from));
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (at[u] + kBytes <= bytes) *reinterpret_cast<V *>(col[u] + to) = v[u];
+                if constexpr (kBytes > 4) {          // a row that ends inside the column
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        for (int j = 0; at[u] < bytes && at[u] + kBytes > bytes && at[u] + j < bytes; j += 4)
+                            *reinterpret_cast<uint32_t *>(col[u] + to + j) = *reinterpret_cast<const uint32_t *>(col[u] + from + j);
+                }
+            }
+        } else {
+            for (int u = 0; u < U; u++) {
+                if (i0 + (long)u * stride >= total) break;
+                for (int j = 0; j < kBytes; j += 4) {
+                    uint32_t kept = 0;
+                    for (int k = 0; k < m.n; k++) {
+                        if (at[u] + j >= m.bytes[k] || at[u] + j >= s.rows * s.row_bytes) continue;
+                        volatile uint32_t *to = reinterpret_cast<uint32_t *>(col[u] + j + max(m.to[k], 0) * s.seq_stride);
+                        const volatile uint32_t *from = reinterpret_cast<const uint32_t *>(col[u] + j + max(m.from[k], 0) * s.seq_stride);
+                        if (m.to[k] < 0) kept = *from;
+                        else *to = m.from[k] < 0 ? kept : *from;
+                    }
+                }
+            }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const ReorderArgs a) {
+    __shared__ Moves m;
+    __shared__ int s_parent[kMaxBeams], s_bytes[kMaxBeams], s_most;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int parent[W], used[W];
-    const int g = blockIdx.y;
-    bool bad = false;
+    const int g = blockIdx.y, lane = threadIdx.x & 31;
     int k = 0;
     while (k + 1 < a.n_states && (int)blockIdx.x >= a.state[k + 1].first) k++;
-    const ReorderState &s = a.state[k];
-    int most = 0;
-#pragma unroll
-    for (int b = 0; b < W; b++) {
-        parent[b] = b;
-        used[b] = 0;
-        if (b < a.width) {
-            const int p = a.parents[g * a.width + b];
-            if ((unsigned)p < (unsigned)a.width) parent[b] = p;
-            else bad = true;
+    const ReorderState s = a.state[k];
+    if (threadIdx.x < 32) {
+        int parent = lane, bytes = 0;
+        bool bad = false;
+        if (lane < a.width) {
+            const int p = a.parents[g * a.width + lane];
+            bad = (unsigned)p >= (unsigned)a.width;
+            if (!bad) parent = p;
             int n = s.rows;
-            if (a.lengths) {
-                n = max(a.lengths[g * a.width + parent[b]], 0);
+            if (parent != lane && a.lengths) {
+                n = max(a.lengths[g * a.width + parent], 0);
                 if (s.mod) n %= s.mod;
                 n = min(n / s.per_row + (n % s.per_row != 0), s.rows);
             }
-            used[b] = parent[b] == b ? 0 : n;
-            most = max(most, used[b]);
+            if (parent == lane) n = 0;
+            bytes = n * s.row_bytes;
+            s_parent[lane] = parent;
+            s_bytes[lane] = bytes;
+        }
+        if (__any_sync(kFullMask, bad) && a.status && lane == 0) atomicOr(a.status, 32u);
+        const bool moves = parent != lane && bytes > 0;
+        const unsigned moving = __ballot_sync(kFullMask, moves), sources = __reduce_or_sync(kFullMask, parent != lane ? 1u << parent : 0u);
+        const bool hazard = __any_sync(kFullMask, parent != lane && (sources >> lane & 1));
+        if (moves) {
+            const int at = __popc(moving & ((1u << lane) - 1));
+            m.to[at] = lane; m.from[at] = parent; m.bytes[at] = bytes;
+        }
+        const int most = __reduce_max_sync(kFullMask, bytes);
+        __syncwarp();
+        if (lane == 0) {
+            m.n = __popc(moving);
+            m.ordered = hazard;
+            s_most = most;
+            if (hazard) order_moves(m, s_parent, s_bytes, a.width);
         }
     }
-    if (bad && a.status && threadIdx.x == 0) atomicOr(a.status, 32u);
+    __syncthreads();
     const int ctas = (k + 1 < a.n_states ? a.state[k + 1].first : (int)gridDim.x) - s.first, cta = blockIdx.x - s.first;
-    const long per_outer = ((long)most * s.row_bytes + s.vec - 1) / s.vec, total = per_outer * s.outer;
+    const int vec = s.wide ? 16 : 4, per_outer = (s_most + vec - 1) / vec;
+    if (per_outer == 0) return;
     uint8_t *base = s.base + (long)g * a.width * s.seq_stride;
-    for (long i = (long)cta * kReorderThreads + threadIdx.x; i < total; i += (long)ctas * kReorderThreads) {
-        const long o = i / per_outer, at = (i - o * per_outer) * s.vec;
-        uint8_t *col = base + o * s.outer_stride + at;
-        // a row whose parent is filled less far than another's is copied up to there only, in words
-        int from[W];
-        bool whole = true;
-#pragma unroll
-        for (int b = 0; b < W; b++) {
-            const long left = (long)used[b] * s.row_bytes - at;
-            from[b] = left > 0 ? parent[b] : b;
-            whole &= left <= 0 || left >= s.vec;
-        }
-        if (s.vec == 16 && whole) reorder_column<W, uint4>(col, s.seq_stride, from, a.width);
-        else {
-            for (int j = 0; j < s.vec; j += 4) {
-#pragma unroll
-                for (int b = 0; b < W; b++) from[b] = (long)used[b] * s.row_bytes - at > j ? parent[b] : b;
-                reorder_column<W, uint32_t>(col + j, s.seq_stride, from, a.width);
-            }
-        }
-    }
+    if (s.wide) copy_columns<uint4>(s, m, base, per_outer, per_outer * s.outer, cta, ctas);
+    else copy_columns<uint32_t>(s, m, base, per_outer, per_outer * s.outer, cta, ctas);
 }
 
 }  // namespace
@@ -389,9 +466,10 @@ extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, co
             return QTIP_ERR_BAD_SHAPE;
         if (!aligned(s.base, 4)) return QTIP_ERR_ALIGNMENT;
         const bool wide = aligned(s.base, 16) && !(s.seq_stride & 15) && (s.outer == 1 || !(s.outer_stride & 15));
-        a.state[k] = {static_cast<uint8_t *>(s.base), s.seq_stride, s.outer_stride, s.outer, s.row_bytes, s.rows, s.per_row, s.mod, wide ? 16 : 4, ctas};
-        const long units = ((long)s.rows * s.row_bytes + a.state[k].vec - 1) / a.state[k].vec * s.outer;
-        const long want = (units + kReorderThreads - 1) / kReorderThreads, most = (long)sm_count() * 8;
+        const long piece = (long)s.rows * s.row_bytes, units = (piece + (wide ? 15 : 3)) / (wide ? 16 : 4) * s.outer;
+        if (piece > 0x3FFFFFFF || units > 0x3FFFFFFF) return QTIP_ERR_TOO_LARGE;        // columns and bytes of a piece are counted in 32 bits
+        a.state[k] = {static_cast<uint8_t *>(s.base), s.seq_stride, s.outer_stride, s.outer, s.row_bytes, s.rows, s.per_row, s.mod, ctas, wide};
+        const long want = (units + kReorderThreads * kReorderColumns - 1) / (kReorderThreads * kReorderColumns), most = (long)sm_count() * 8;
         ctas += (int)(want < most ? want : most);
     }
     if (width == 1) return QTIP_OK;
@@ -404,8 +482,6 @@ extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, co
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (width <= 4) QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel<4>, a));
-    else if (width <= 8) QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel<8>, a));
-    else QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel<16>, a));
+    QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel, a));
     return check_launch();
 }

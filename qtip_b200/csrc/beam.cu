@@ -62,27 +62,41 @@ __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 template <typename T>
 __device__ __forceinline__ void load_batch(float (&x)[kSelectHeld], const T *row, int base, int end, int lane, bool vectors) {
     constexpr int N = Vec<T>::n;
-    if (vectors && base + 32 * kSelectHeld <= end) {
 #pragma unroll
-        for (int j = 0; j < kSelectHeld / N; j++) {
-            const typename Vec<T>::type v = __ldcs(reinterpret_cast<const typename Vec<T>::type *>(row + base + (j * 32 + lane) * N));
-            const T *e = reinterpret_cast<const T *>(&v);
+    for (int j = 0; j < kSelectHeld / N; j++) {
+        const int at = base + (j * 32 + lane) * N;
+        typename Vec<T>::type v;
+        T *e = reinterpret_cast<T *>(&v);
+        if (vectors && at + N <= end) v = __ldcs(reinterpret_cast<const typename Vec<T>::type *>(row + at));
+        else {
 #pragma unroll
-            for (int k = 0; k < N; k++) x[j * N + k] = to_f(e[k]);
+            for (int k = 0; k < N; k++) e[k] = at + k < end ? row[at + k] : T(-INFINITY);
         }
-    } else {
 #pragma unroll
-        for (int j = 0; j < kSelectHeld / N; j++)
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                const int i = base + (j * 32 + lane) * N + k;
-                x[j * N + k] = i < end ? to_f(row[i]) : -INFINITY;
-            }
+        for (int k = 0; k < N; k++) x[j * N + k] = to_f(e[k]);
     }
 }
 
+// Sum of exp(x - m) of a batch, m brought up to the batch's largest; NaN where the batch holds an infinity or NaN.
+__device__ __forceinline__ float batch_sum(const float (&x)[kSelectHeld], float &m, float &sum, float &top) {
+    top = x[0];
+#pragma unroll
+    for (int j = 1; j < kSelectHeld; j++) top = fmaxf(top, x[j]);
+    const float up = fmaxf(m, top), at = up == -INFINITY ? 0.f : up;
+    sum *= exp2f((m - at) * 1.4426950408889634f);
+    m = up;
+    float s[4] = {};
+#pragma unroll
+    for (int j = 0; j < kSelectHeld; j++) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[j] - at) * 1.4426950408889634f));
+        s[j & 3] += e;
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kSelectThreads) beam_select_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kSelectThreads, 2) beam_select_kernel(const SelectArgs a) {
     constexpr int N = Vec<T>::n;
     __shared__ SelectSmem S;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.width, g = blockIdx.y;
@@ -103,47 +117,55 @@ __global__ void __launch_bounds__(kSelectThreads) beam_select_kernel(const Selec
         const long long lo = (long long)part * slice;
         const int end = (int)min((long long)a.vocab, lo + slice);
         for (long long at = lo; at < end && !dead; at += 32 * kSelectHeld) {
-            float x[kSelectHeld], top = -INFINITY;
+            float x[kSelectHeld], top;
             load_batch<T>(x, row, (int)at, end, lane, vectors);
+            const float m0 = m, sum0 = sum;
+            float more = batch_sum(x, m, sum, top);
+            if (__any_sync(kFullMask, !(more <= 3.0e38f))) {           // something that is not a finite number: it does not count
+                m = m0;
+                sum = sum0;
 #pragma unroll
-            for (int j = 0; j < kSelectHeld; j++) {
-                if (!isfinite(x[j])) x[j] = -INFINITY;
-                top = fmaxf(top, x[j]);
+                for (int j = 0; j < kSelectHeld; j++)
+                    if (!isfinite(x[j])) x[j] = -INFINITY;
+                more = batch_sum(x, m, sum, top);
             }
-            if (top > m) {
-                sum *= exp2f((m - top) * 1.4426950408889634f);         // (m = -inf: 0 times 0)
-                m = top;
+            sum += more;
+            // what can enter the list: not below its last entry; in the first batch not below the W-th largest of the lanes' largest
+            uint32_t bound = (uint32_t)(__shfl_sync(kFullMask, list, W - 1) >> 32);
+            if (bound == 0u) {
+                uint32_t mine = top > -INFINITY ? ordered(top) : 0u;
+                for (int r = 0; r < W; r++) {
+                    bound = __reduce_max_sync(kFullMask, mine);
+                    const unsigned who = __ballot_sync(kFullMask, mine == bound);
+                    if (lane == __ffs(who) - 1) mine = 0u;
+                }
             }
-            if (m > -INFINITY) {
+            const float least = bound ? unordered(bound) : -INFINITY;
+            if (!__any_sync(kFullMask, top >= least && top > -INFINITY)) continue;
+            unsigned open = 0;
 #pragma unroll
-                for (int j = 0; j < kSelectHeld; j++) sum += exp2f((x[j] - m) * 1.4426950408889634f);
-            }
-            // the W-th largest of the lanes' largest bounds what can enter the list
-            uint32_t mine = top > -INFINITY ? ordered(top) : 0u, bound = 0u;
-            for (int r = 0; r < W; r++) {
-                bound = __reduce_max_sync(kFullMask, mine);
-                const unsigned who = __ballot_sync(kFullMask, mine == bound);
-                if (lane == __ffs(who) - 1) mine = 0u;
-            }
-            bound = max(bound, (uint32_t)(__shfl_sync(kFullMask, list, W - 1) >> 32));
-            if (!__ballot_sync(kFullMask, top > -INFINITY && ordered(top) >= bound)) continue;
-#pragma unroll 1
-            for (int j = 0; j < kSelectHeld; j++) {
-                float v = -INFINITY;
+            for (int j = 0; j < kSelectHeld; j++) open |= x[j] >= least && x[j] > -INFINITY ? 1u << j : 0u;
+            while (__any_sync(kFullMask, open != 0u)) {
+                // every lane's next one, then one lane after the other
+                const int j = open ? __ffs(open) - 1 : 0;
+                float pick[kSelectHeld / 2];
 #pragma unroll
-                for (int q = 0; q < kSelectHeld; q++) v = q == j ? x[q] : v;
+                for (int q = 0; q < kSelectHeld / 2; q++) pick[q] = j & 1 ? x[2 * q + 1] : x[2 * q];
+#pragma unroll
+                for (int step = 1; step < kSelectHeld / 2; step <<= 1)
+#pragma unroll
+                    for (int q = 0; q < kSelectHeld / 2; q += 2 * step) pick[q] = j & (2 * step) ? pick[q + step] : pick[q];
                 const uint32_t idx = (uint32_t)((int)at + ((j / N) * 32 + lane) * N + j % N);
-                const unsigned long long key = v > -INFINITY ? (unsigned long long)ordered(v) << 32 | (0xFFFFFFFFu - idx) : 0ull;
-                bool open = (uint32_t)(key >> 32) >= bound && key != 0ull;
-                for (;;) {
-                    const unsigned long long last = __shfl_sync(kFullMask, list, W - 1);
-                    open = open && key > last;
-                    const unsigned who = __ballot_sync(kFullMask, open);
-                    if (!who) break;
+                const unsigned long long key = open ? (unsigned long long)ordered(pick[0]) << 32 | (0xFFFFFFFFu - idx) : 0ull;
+                open &= open - 1;
+                unsigned long long last = __shfl_sync(kFullMask, list, W - 1);
+                unsigned who = __ballot_sync(kFullMask, key > last);
+                while (who) {
                     const int src = __ffs(who) - 1;
                     const unsigned long long k = __shfl_sync(kFullMask, key, src), up = __shfl_up_sync(kFullMask, list, 1);
                     if (k > list) list = lane == 0 || up > k ? k : up;
-                    if (lane == src) open = false;
+                    last = __shfl_sync(kFullMask, list, W - 1);
+                    who = __ballot_sync(kFullMask, key > last) & who & (who - 1);
                 }
             }
         }

@@ -9,10 +9,11 @@ constexpr int kMaxBeams = 16, kMaxStates = 8;
 
 // ---- selection -------------------------------------------------------------------------------------------------------------------
 // A group's beams w < W with scores c_w and logits x_w: the W largest of c_w + (x_wv - lse_w), lse_w = log sum_v exp x_wv.
-// One cluster per group; its 128 warps share the rows.  A warp reads its slice once: the sum of exponentials with a running maximum in each
-// lane, and the W largest logits, which lie sorted in its lanes (a logit that is not above the last of them costs one comparison).  CTA 0
+// One cluster per group; its warps share the rows.  A warp reads its slice once, in batches of 32 logits per lane that are copied to shared memory
+// one batch ahead: the sum of exponentials with a running maximum in each lane, and the W largest logits, sorted in its lanes.  A batch without
+// a logit above the last of these costs one comparison; in the first batch the W-th largest of the lanes' largest is the bound.  CTA 0
 // merges the lists of a row, one warp per row, adds scores in 64 bits and takes the W largest of the W * W continuations that are left.
-constexpr int kSelectThreads = 512, kSelectCluster = 8, kSelectWarps = kSelectThreads / 32 * kSelectCluster, kSelectHeld = 32;
+constexpr int kSelectThreads = 256, kSelectCluster = 16, kSelectWarps = kSelectThreads / 32 * kSelectCluster, kSelectHeld = 32, kSelectStages = 2;
 
 struct SelectArgs {
     long long *tokens;
@@ -29,7 +30,7 @@ struct SelectArgs {
 
 struct SelectSmem {
     unsigned long long keys[kSelectWarps * kMaxBeams];       // (row, warp of the row, rank)
-    float2 sums[kSelectWarps];                               // (row, warp of the row): maximum, sum of exponentials
+    float2 sums[kSelectWarps];                               // (row, warp of the row): unit, sum of exponentials
     unsigned long long total[kMaxBeams * kMaxBeams];         // ordered bits of the continuations' scores; 0: none
     int token[kMaxBeams * kMaxBeams];
 };
@@ -52,62 +53,95 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
     return (unsigned long long)hi << 32 | lo;
 }
 
-template <typename T> struct Vec;
-template <> struct Vec<float> { using type = float4; static constexpr int n = 4; };
-template <> struct Vec<__half> { using type = uint4; static constexpr int n = 8; };
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 
-// One batch of a lane's logits: x[j] is that of index base + place(j), -inf where there is none.
+// Exponentials are powers of two of x * kLog2e less a whole number, so that only the last sum is rounded.  The logarithm, divided by the same
+// constant, is off by its relative rounding (1.3e-8) times the entropy of the row.
+constexpr float kLog2e = 1.44269502162933349609375f;
+
+// A warp's batch in shared memory: vector j of lane l holds logits base + (j * 32 + l) * N + k; -inf behind the end of the slice.  A lane reads what
+// it copied itself.
 template <typename T>
-__device__ __forceinline__ void load_batch(float (&x)[kSelectHeld], const T *row, int base, int end, int lane, bool vectors) {
-    constexpr int N = Vec<T>::n;
+struct Batch {
+    static constexpr int N = 16 / sizeof(T), V = kSelectHeld / N, kSize = 32 * kSelectHeld;
+    uint4 v[V][32];
+    __device__ __forceinline__ void load(const T *row, int base, int end, int lane, bool vectors) {
+        if (vectors && base + kSize <= end) copy<true>(row, base, end, lane, true);
+        else copy<false>(row, base, end, lane, vectors);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    template <bool whole>
+    __device__ __forceinline__ void copy(const T *row, int base, int end, int lane, bool vectors) {
 #pragma unroll
-    for (int j = 0; j < kSelectHeld / N; j++) {
-        const int at = base + (j * 32 + lane) * N;
-        typename Vec<T>::type v;
-        T *e = reinterpret_cast<T *>(&v);
-        if (vectors && at + N <= end) v = __ldcs(reinterpret_cast<const typename Vec<T>::type *>(row + at));
-        else {
+        for (int j = 0; j < V; j++) {
+            const int at = base + (j * 32 + lane) * N;
+            if (vectors && (whole || at + N <= end)) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&v[j][lane])), "l"(row + at) : "memory");
+            } else {
+                T *e = reinterpret_cast<T *>(&v[j][lane]);
 #pragma unroll
-            for (int k = 0; k < N; k++) e[k] = at + k < end ? row[at + k] : T(-INFINITY);
+                for (int k = 0; k < N; k++) e[k] = at + k < end ? row[at + k] : T(-INFINITY);
+            }
         }
-#pragma unroll
-        for (int k = 0; k < N; k++) x[j * N + k] = to_f(e[k]);
     }
-}
-
-// Sum of exp(x - m) of a batch, m brought up to the batch's largest; NaN where the batch holds an infinity or NaN.
-__device__ __forceinline__ float batch_sum(const float (&x)[kSelectHeld], float &m, float &sum, float &top) {
-    top = x[0];
+    __device__ __forceinline__ void values(float (&x)[N], int j, int lane) const {
+        const uint4 raw = v[j][lane];
 #pragma unroll
-    for (int j = 1; j < kSelectHeld; j++) top = fmaxf(top, x[j]);
-    const float up = fmaxf(m, top), at = up == -INFINITY ? 0.f : up;
-    sum *= exp2f((m - at) * 1.4426950408889634f);
-    m = up;
-    float s[4] = {};
-#pragma unroll
-    for (int j = 0; j < kSelectHeld; j++) {
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[j] - at) * 1.4426950408889634f));
-        s[j & 3] += e;
+        for (int k = 0; k < N; k++) x[k] = to_f(reinterpret_cast<const T *>(&raw)[k]);
     }
-    return (s[0] + s[1]) + (s[2] + s[3]);
-}
+    __device__ __forceinline__ float value(int i, int lane) const { return to_f(reinterpret_cast<const T *>(&v[i / N][lane])[i % N]); }
+    __device__ __forceinline__ float largest(int lane) const {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float x[N];
+            values(x, j, lane);
+#pragma unroll
+            for (int k = 0; k < N; k++) top = fmaxf(top, x[k]);
+        }
+        return top;
+    }
+    // Sum of 2^(x * kLog2e - unit), and the largest.
+    __device__ __forceinline__ float sum(float unit, float &top, int lane) const {
+        float s[4] = {}, t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float x[N];
+            values(x, j, lane);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                float e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(x[k], kLog2e, -unit)));
+                s[k & 3] += e;
+                t[k & 3] = fmaxf(t[k & 3], x[k]);
+            }
+        }
+        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        return (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    __device__ __forceinline__ void only_finite(int lane) {
+        for (int j = 0; j < V; j++)
+            for (int k = 0; k < N; k++) {
+                T *e = reinterpret_cast<T *>(&v[j][lane]) + k;
+                if (!isfinite(to_f(*e))) *e = T(-INFINITY);
+            }
+    }
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kSelectThreads, 2) beam_select_kernel(const SelectArgs a) {
-    constexpr int N = Vec<T>::n;
-    __shared__ SelectSmem S;
+__global__ void __launch_bounds__(kSelectThreads, 3) beam_select_kernel(const SelectArgs a) {
+    extern __shared__ __align__(16) uint8_t select_smem[];
+    SelectSmem &S = *reinterpret_cast<SelectSmem *>(select_smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.width, g = blockIdx.y;
+    Batch<T> *ring = reinterpret_cast<Batch<T> *>(select_smem) + warp * kSelectStages;
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");      // awaited before the first remote store
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int per = kSelectWarps / W, id = (int)rank * (kSelectThreads / 32) + warp, w = id / per, part = id % per;
+    const int per = (int)gridDim.x * (kSelectThreads / 32) / W, id = (int)rank * (kSelectThreads / 32) + warp, w = id / per, part = id % per;
     unsigned long long list = 0;                             // lane i < W: the i-th largest (logit, ~index)
-    float m = -INFINITY, sum = 0.f;
+    float unit = -INFINITY, sum = 0.f;
     if (w < W) {
         const size_t beam = (size_t)g * W + w;
         const T *row = static_cast<const T *>(a.logits) + beam * (size_t)a.stride;
@@ -116,18 +150,31 @@ __global__ void __launch_bounds__(kSelectThreads, 2) beam_select_kernel(const Se
         const int slice = ((a.vocab + per - 1) / per + 7) & ~7;
         const long long lo = (long long)part * slice;
         const int end = (int)min((long long)a.vocab, lo + slice);
-        for (long long at = lo; at < end && !dead; at += 32 * kSelectHeld) {
-            float x[kSelectHeld], top;
-            load_batch<T>(x, row, (int)at, end, lane, vectors);
-            const float m0 = m, sum0 = sum;
-            float more = batch_sum(x, m, sum, top);
-            if (__any_sync(kFullMask, !(more <= 3.0e38f))) {           // something that is not a finite number: it does not count
-                m = m0;
-                sum = sum0;
-#pragma unroll
-                for (int j = 0; j < kSelectHeld; j++)
-                    if (!isfinite(x[j])) x[j] = -INFINITY;
-                more = batch_sum(x, m, sum, top);
+        int stage = 0;
+        if (lo < end && !dead) ring[0].load(row, (int)lo, end, lane, vectors);
+        for (long long at = lo; at < end && !dead; at += Batch<T>::kSize) {
+            Batch<T> &x = ring[stage];
+            stage ^= 1;
+            if (at + Batch<T>::kSize < end) {                          // in flight during this one
+                ring[stage].load(row, (int)at + Batch<T>::kSize, end, lane, vectors);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            // a lane's unit comes from its first finite logit's batch; a later one is above it by no more than fp32 can hold, or changes it
+            float top;
+            if (__any_sync(kFullMask, unit == -INFINITY)) {
+                top = x.largest(lane);
+                if (unit == -INFINITY && fabsf(top) < INFINITY) unit = ceilf(top * kLog2e);
+            }
+            float more = x.sum(unit == -INFINITY ? 0.f : unit, top, lane);
+            if (__any_sync(kFullMask, !(more <= 3.0e38f))) {           // an infinity or NaN, which do not count, or a change of the unit
+                x.only_finite(lane);
+                top = x.largest(lane);
+                const float old = unit;
+                if (top > -INFINITY) unit = fmaxf(unit, ceilf(top * kLog2e));
+                if (old > -INFINITY) sum *= exp2f(old - unit);
+                more = x.sum(unit == -INFINITY ? 0.f : unit, top, lane);
             }
             sum += more;
             // what can enter the list: not below its last entry; in the first batch not below the W-th largest of the lanes' largest
@@ -143,41 +190,44 @@ __global__ void __launch_bounds__(kSelectThreads, 2) beam_select_kernel(const Se
             const float least = bound ? unordered(bound) : -INFINITY;
             if (!__any_sync(kFullMask, top >= least && top > -INFINITY)) continue;
             unsigned open = 0;
+            if (top >= least) {
 #pragma unroll
-            for (int j = 0; j < kSelectHeld; j++) open |= x[j] >= least && x[j] > -INFINITY ? 1u << j : 0u;
+                for (int j = 0; j < Batch<T>::V; j++) {
+                    float y[Batch<T>::N];
+                    x.values(y, j, lane);
+#pragma unroll
+                    for (int k = 0; k < Batch<T>::N; k++) open |= y[k] >= least && y[k] > -INFINITY ? 1u << (j * Batch<T>::N + k) : 0u;
+                }
+            }
+            __syncwarp();
             while (__any_sync(kFullMask, open != 0u)) {
                 // every lane's next one, then one lane after the other
                 const int j = open ? __ffs(open) - 1 : 0;
-                float pick[kSelectHeld / 2];
-#pragma unroll
-                for (int q = 0; q < kSelectHeld / 2; q++) pick[q] = j & 1 ? x[2 * q + 1] : x[2 * q];
-#pragma unroll
-                for (int step = 1; step < kSelectHeld / 2; step <<= 1)
-#pragma unroll
-                    for (int q = 0; q < kSelectHeld / 2; q += 2 * step) pick[q] = j & (2 * step) ? pick[q + step] : pick[q];
-                const uint32_t idx = (uint32_t)((int)at + ((j / N) * 32 + lane) * N + j % N);
-                const unsigned long long key = open ? (unsigned long long)ordered(pick[0]) << 32 | (0xFFFFFFFFu - idx) : 0ull;
+                const uint32_t idx = (uint32_t)((int)at + ((j / Batch<T>::N) * 32 + lane) * Batch<T>::N + j % Batch<T>::N);
+                const unsigned long long key = open ? (unsigned long long)ordered(x.value(j, lane)) << 32 | (0xFFFFFFFFu - idx) : 0ull;
                 open &= open - 1;
                 unsigned long long last = __shfl_sync(kFullMask, list, W - 1);
                 unsigned who = __ballot_sync(kFullMask, key > last);
                 while (who) {
                     const int src = __ffs(who) - 1;
-                    const unsigned long long k = __shfl_sync(kFullMask, key, src), up = __shfl_up_sync(kFullMask, list, 1);
-                    if (k > list) list = lane == 0 || up > k ? k : up;
+                    const unsigned long long k = __shfl_sync(kFullMask, key, src), before = __shfl_up_sync(kFullMask, list, 1);
+                    if (k > list) list = lane == 0 || before > k ? k : before;
                     last = __shfl_sync(kFullMask, list, W - 1);
                     who = __ballot_sync(kFullMask, key > last) & who & (who - 1);
                 }
             }
         }
         // the lanes' sums
-        float all = m;
+        float all = unit;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFullMask, all, o));
-        sum = m > -INFINITY ? sum * exp2f((m - all) * 1.4426950408889634f) : 0.f;
+        sum = unit > -INFINITY ? sum * exp2f(unit - all) : 0.f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-        m = all;
+        unit = all;
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");      // the lists take the place of the batches
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (w < W) {
         uint32_t to;
@@ -187,33 +237,33 @@ __global__ void __launch_bounds__(kSelectThreads, 2) beam_select_kernel(const Se
         }
         if (lane == 0) {
             asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&S.sums[id])));
-            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(m), "f"(sum) : "memory");
+            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(unit), "f"(sum) : "memory");
         }
     }
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     if (rank != 0) return;
-    if (warp < W) {
-        const size_t beam = (size_t)g * W + warp;
+    for (int row = warp; row < W; row += kSelectThreads / 32) {
+        const size_t beam = (size_t)g * W + row;
         const float score = a.prev_scores[beam];
         const bool active = isfinite(score), ended = a.eos >= 0 && a.prev_tokens && a.prev_tokens[beam] == a.eos;
         // log of the row's sum: terms of 32 bits, added in 64
         float mx = -INFINITY;
-        for (int i = lane; i < per; i += 32) mx = fmaxf(mx, S.sums[warp * per + i].x);
+        for (int i = lane; i < per; i += 32) mx = fmaxf(mx, S.sums[row * per + i].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
         double s = 0.0;
         for (int i = lane; i < per; i += 32) {
-            const float2 v = S.sums[warp * per + i];
-            if (v.y > 0.f) s += (double)v.y * (double)exp2f((v.x - mx) * 1.4426950408889634f);
+            const float2 v = S.sums[row * per + i];
+            if (v.y > 0.f) s += (double)v.y * (double)exp2f(v.x - mx);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-        const double lse = (double)(float)((double)mx + log(s));
+        const double lse = (double)(float)(((double)mx + log2(s)) / (double)kLog2e);
         unsigned long long k[kSelectWarps / 32];
 #pragma unroll
         for (int e = 0; e < kSelectWarps / 32; e++) {
             const int i = lane + 32 * e;
-            k[e] = i < per * W ? S.keys[warp * per * W + i] : 0ull;
+            k[e] = i < per * W ? S.keys[row * per * W + i] : 0ull;
         }
         for (int r = 0; r < W; r++) {
             unsigned long long best = k[0];
@@ -232,8 +282,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) beam_select_kernel(const Se
                 } else if (active && best != 0ull) {
                     total = ordered((double)score + ((double)unordered((uint32_t)(best >> 32)) - lse));
                 }
-                S.total[warp * W + r] = total;
-                S.token[warp * W + r] = token;
+                S.total[row * W + r] = total;
+                S.token[row * W + r] = token;
             }
         }
     }
@@ -439,6 +489,56 @@ __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const Reo
     else copy_columns<uint32_t>(s, m, base, per_outer, per_outer * s.outer, cta, ctas);
 }
 
+template <typename T>
+constexpr size_t select_smem_bytes() {
+    constexpr size_t ring = (size_t)kSelectThreads / 32 * kSelectStages * sizeof(Batch<T>);
+    return ring > sizeof(SelectSmem) ? ring : sizeof(SelectSmem);
+}
+
+// CTAs of a group: 1 to 16 (8 where the GPU has no room for clusters of 16), so that the rounds of clusters that the chip holds at once, each as long
+// as a warp's part of a row, take the least time.
+template <typename T>
+int launch_select(const SelectArgs &a, int groups, cudaStream_t stream) {
+    static int cached[64][5] = {};       // clusters of 1, 2, 4, 8, 16 CTAs at once, plus one
+    int dev = 0, cluster = 0;
+    QTIP_CUDA_TRY(cudaGetDevice(&dev));
+    QTIP_CUDA_TRY(cudaFuncSetAttribute(beam_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)select_smem_bytes<T>()));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = select_smem_bytes<T>();
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    double best = 0;
+    for (int k = 0; k < 5; k++) {
+        const int c = 1 << k, per = c * (kSelectThreads / 32) / a.width;                   // warps of a row
+        if (per == 0) continue;
+        int n = dev < 64 ? cached[dev][k] - 1 : -1;
+        if (n < 0) {
+            cfg.gridDim = dim3(c);
+            cfg.numAttrs = 1;
+            attr[0].val.clusterDim.x = c;
+            if ((c == 16 && cudaFuncSetAttribute(beam_select_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+                cudaOccupancyMaxActiveClusters(&n, beam_select_kernel<T>, &cfg) != cudaSuccess) {
+                (void)cudaGetLastError();
+                n = 0;
+            }
+            if (dev < 64) cached[dev][k] = n + 1;
+        }
+        const double time = n ? (double)((groups + n - 1) / n) / per : 1e30;
+        if (!cluster || time < best) { cluster = c; best = time; }
+    }
+    cfg.gridDim = dim3(cluster, groups);
+    cfg.numAttrs = 2;
+    attr[0].val.clusterDim.x = cluster;
+    QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_select_kernel<T>, a));
+    return check_launch();
+}
+
 }  // namespace
 }  // namespace qtip
 
@@ -451,22 +551,8 @@ extern "C" int qtip_beam_select(long long *tokens, int *parents, float *scores, 
         return QTIP_ERR_BAD_ARG;
     if (groups < 1 || groups > 65535 || width < 1 || width > kMaxBeams || vocab < 1 || vocab > (1 << 30) || logits_stride < vocab) return QTIP_ERR_BAD_SHAPE;
     const SelectArgs a = {tokens, parents, scores, logits, logits_stride, prev_scores, prev_tokens, width, vocab, eos, status};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kSelectCluster, groups);
-    cfg.blockDim = dim3(kSelectThreads);
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = kSelectCluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if (logits_dtype == QTIP_F32) QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_select_kernel<float>, a));
-    else QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_select_kernel<__half>, a));
-    return check_launch();
+    return logits_dtype == QTIP_F32 ? launch_select<float>(a, groups, static_cast<cudaStream_t>(stream))
+                                    : launch_select<__half>(a, groups, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, const int *parents, const int *lengths, int groups, int width,

@@ -12,7 +12,7 @@ namespace {
 // One CTA.  A block is free when no sequence's table names it among its complete blocks (a bitmap in shared memory): there is no free
 // list to keep, a sequence whose length is set to zero has released its blocks, and tables that name the same block (beams of one
 // search, a common prompt) share it.  The new blocks are the lowest free ones, in the order of the sequences.
-constexpr int kPlanThreads = 1024, kPlanMaxBlocks = 1600000, kPlanMaxTokens = 1 << 20;
+constexpr int kPlanThreads = 1024, kPlanLoads = 8, kPlanMaxBlocks = 1600000, kPlanMaxTokens = 1 << 20;
 
 struct PlanArgs {
     int *tables;
@@ -50,6 +50,8 @@ __device__ __forceinline__ int block_scan(int v, int *sums, int &total) {
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a) {
     extern __shared__ uint32_t held[];                       // a bit per block of the pool
     __shared__ int sums[33], s_len[kPlanThreads], s_new[kPlanThreads], s_base[kPlanThreads], s_run[kPlanThreads], s_tok[kPlanThreads], s_free[kPlanThreads];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = a.block;
     const int words = (a.n_blocks + 31) >> 5, per = (words + kPlanThreads - 1) / kPlanThreads;
     unsigned bad = 0;
@@ -60,10 +62,17 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
     __syncthreads();
     for (int s = warp; s < a.n_seqs; s += kPlanThreads / 32) {
         const int live = min(max(a.lengths[s], 0) / b, a.max_blocks);
-        for (int j = lane; j < live; j += 32) {
-            const int id = a.tables[(size_t)s * a.max_blocks + j];
-            if ((unsigned)id < (unsigned)a.n_blocks) atomicOr(&held[id >> 5], 1u << (id & 31));
-            else bad |= 16u;
+        const int *row = a.tables + (size_t)s * a.max_blocks;
+        for (int j0 = lane; j0 < live; j0 += 32 * kPlanLoads) {      // the loads of a step are in flight together
+            int id[kPlanLoads];
+#pragma unroll
+            for (int u = 0; u < kPlanLoads; u++) id[u] = j0 + 32 * u < live ? row[j0 + 32 * u] : 0;
+#pragma unroll
+            for (int u = 0; u < kPlanLoads; u++) {
+                if (j0 + 32 * u >= live) break;
+                if ((unsigned)id[u] < (unsigned)a.n_blocks) atomicOr(&held[id[u] >> 5], 1u << (id[u] & 31));
+                else bad |= 16u;
+            }
         }
     }
     __syncthreads();
@@ -106,36 +115,41 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
         s_tok[tid] = (int)tok;
         if (in) a.lengths_out[s] = len + fresh;
         __syncthreads();
-        for (int q = warp; q < count; q += kPlanThreads / 32) {
-            const int L = s_len[q], n = s_new[q];
-            if (n == 0) continue;
-            const int first = L / b, end = L + n, nr = (end - 1) / b - first + 1;
-            const bool shared = L % b != 0 && nr > 1 && end % b != 0;
-            for (int i = lane; i < nr; i += 32) {
-                const int pos0 = i == 0 ? L : (first + i) * b, stop = min((first + i + 1) * b, end);
-                int id = -1;
-                if (stop % b == 0) {
-                    // the free block of rank s_base + i: the thread whose words hold it, then the word, then the bit
-                    const int rank = s_base[q] + i;
-                    int lo = 0, hi = kPlanThreads - 1;
-                    while (lo < hi) {
-                        const int mid = (lo + hi) >> 1;
-                        if (s_free[mid] > rank) hi = mid;
-                        else lo = mid + 1;
-                    }
-                    int left = rank - (lo ? s_free[lo - 1] : 0), w = lo * per;
-                    for (; w < words; w++) {
-                        const int c = 32 - __popc(held[w]);
-                        if (left < c) break;
-                        left -= c;
-                    }
-                    id = w * 32 + (int)__fns(~held[min(w, words - 1)], 0, left + 1);
-                    a.tables[(size_t)(s0 + q) * a.max_blocks + first + i] = id;
-                } else if (shared && i == nr - 1) id = -2;
-                int4 *out = reinterpret_cast<int4 *>(a.runs + (size_t)(s_run[q] + i) * kRunInts);
-                out[0] = make_int4(s0 + q, s_tok[q] + pos0 - L, pos0, stop - pos0);
-                out[1] = make_int4(id, shared && i == 0 ? s_run[q] + nr - 1 : -1, 0, 0);
+        // a run each thread: its sequence is the last that begins not behind it
+        for (int r = run_at - total + tid; r < run_at; r += kPlanThreads) {
+            int q = 0, beyond = count;
+            while (beyond - q > 1) {
+                const int mid = (q + beyond) >> 1;
+                if (s_run[mid] <= r) q = mid;
+                else beyond = mid;
             }
+            const int L = s_len[q], n = s_new[q], i = r - s_run[q], first = L / b, end = L + n, nr = (end - 1) / b - first + 1;
+            const bool shared = L % b != 0 && nr > 1 && end % b != 0;
+            const int pos0 = i == 0 ? L : (first + i) * b, stop = min((first + i + 1) * b, end);
+            int id = -1;
+            if (stop % b == 0) {
+                // the free block of rank s_base + i: the thread whose words hold it, then the word, then the bit
+                const int rank = s_base[q] + i;
+                int lo = 0, hi = kPlanThreads - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_free[mid] > rank) hi = mid;
+                    else lo = mid + 1;
+                }
+                int left = rank - (lo ? s_free[lo - 1] : 0), w = lo * per;
+                for (; w < words; w++) {
+                    const int c = 32 - __popc(held[w]);
+                    if (left < c) break;
+                    left -= c;
+                }
+                uint32_t open = ~held[min(w, words - 1)];
+                for (; left > 0; left--) open &= open - 1;
+                id = w * 32 + __ffs(open) - 1;
+                a.tables[(size_t)(s0 + q) * a.max_blocks + first + i] = id;
+            } else if (shared && i == nr - 1) id = -2;
+            int4 *out = reinterpret_cast<int4 *>(a.runs + (size_t)r * kRunInts);
+            out[0] = make_int4(s0 + q, s_tok[q] + pos0 - L, pos0, stop - pos0);
+            out[1] = make_int4(id, shared && i == 0 ? s_run[q] + nr - 1 : -1, 0, 0);
         }
         __syncthreads();
     }
@@ -158,24 +172,58 @@ struct AppendArgs {
     unsigned *status;
 };
 
-constexpr int kAppendThreads = 256;
+// One CTA per run and share of the heads: all its copies are 16 bytes wide.  Bound by the bytes of q, k and v.  The angle is in 64 bits: at position
+// 10^6 its rounding to 32 would turn a key by 0.03.  The products and sums of the rotation are rounded one by one, as in torch.
+constexpr int kAppendThreads = 256, kAppendUnroll = 4;
+
+struct Turn {
+    float cs[8], sn[8];
+    __device__ __forceinline__ void load(const float2 *t) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float4 v = reinterpret_cast<const float4 *>(t)[j];
+            cs[2 * j] = v.x; sn[2 * j] = v.y; cs[2 * j + 1] = v.z; sn[2 * j + 1] = v.w;
+        }
+    }
+    // dims i .. i + 7 and i + HD/2 .. of one head
+    __device__ __forceinline__ void apply(uint4 &lo, uint4 &hi) const {
+        __half2 *a = reinterpret_cast<__half2 *>(&lo), *b = reinterpret_cast<__half2 *>(&hi);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 x = __half22float2(a[j]), y = __half22float2(b[j]);
+            const float c0 = cs[2 * j], s0 = sn[2 * j], c1 = cs[2 * j + 1], s1 = sn[2 * j + 1];
+            a[j] = __floats2half2_rn(__fsub_rn(__fmul_rn(x.x, c0), __fmul_rn(y.x, s0)), __fsub_rn(__fmul_rn(x.y, c1), __fmul_rn(y.y, s1)));
+            b[j] = __floats2half2_rn(__fadd_rn(__fmul_rn(y.x, c0), __fmul_rn(x.x, s0)), __fadd_rn(__fmul_rn(y.y, c1), __fmul_rn(x.y, s1)));
+        }
+    }
+};
+
+template <int KIND>
+__device__ __forceinline__ uint32_t code_of(float x, bool finite) {
+    if constexpr (KIND == kKvInt8) return finite ? (uint32_t)((int)rintf(x) + 128) : 128u;
+    else return finite ? (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3) : 0u;
+}
 
 template <int HD, int KIND>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+    constexpr int kChunks = HD / 16;                         // pairs of 8 dims of a head
     extern __shared__ __align__(16) uint8_t append_smem[];
-    const int b = a.block, tid = threadIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int b = a.block, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float2 *turn = reinterpret_cast<float2 *>(append_smem);                   // [block][HD/2] cos, sin
-    __half *tile = reinterpret_cast<__half *>(turn + b * (HD / 2));           // [block][HD] one head's rows
-    __shared__ unsigned s_amax;
-    if ((int)blockIdx.x >= *a.n_runs) return;
+    __half *tile = reinterpret_cast<__half *>(turn + b * (HD / 2));           // [block][HD] one head's rows of K or V
+    __shared__ unsigned s_amax[2];
+    const int n_runs = *a.n_runs;
+    if ((int)blockIdx.x >= n_runs) return;
     int run = blockIdx.x, extra = -1;
     const int kv_per = (a.n_kv + gridDim.y - 1) / gridDim.y, kv0 = blockIdx.y * kv_per, kv1 = min(kv0 + kv_per, a.n_kv);
-    const int q_per = (a.n_heads + gridDim.y - 1) / gridDim.y, q0 = blockIdx.y * q_per, q1 = min(q0 + q_per, a.n_heads);
+    const int rep = a.n_heads / a.n_kv, q0 = kv0 * rep, nq = max(kv1 - kv0, 0) * rep;
     for (int part = 0; part < 2; part++) {
         const int4 r0 = reinterpret_cast<const int4 *>(a.runs)[2 * run], r1 = reinterpret_cast<const int4 *>(a.runs)[2 * run + 1];
-        const int seq = r0.x, tok0 = r0.y, pos0 = r0.z, count = r0.w, id = r1.x, o = pos0 % b;
-        if ((unsigned)seq >= (unsigned)a.n_seqs || tok0 < 0 || count < 0 || pos0 < 0 || o + count > b || tok0 + count > a.n_tokens || id >= a.n_blocks ||
-            (id >= 0 && o + count != b)) {
+        const int seq = r0.x, tok0 = r0.y, pos0 = r0.z, count = r0.w, id = r1.x, o = pos0 & (b - 1);
+        if ((unsigned)seq >= (unsigned)a.n_seqs || tok0 < 0 || count < 0 || count > b || pos0 < 0 || o + count > b || tok0 > a.n_tokens - count ||
+            id >= a.n_blocks || (id >= 0 && o + count != b)) {
             if (a.status && tid == 0) atomicOr(a.status, 1u);
             return;
         }
@@ -184,79 +232,145 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
             extra = r1.y;
         }
         __syncthreads();
-        // the angle in 64 bits: at position 10^6 its rounding to 32 would turn a key by 0.03
         for (int i = tid; i < count * (HD / 2); i += kAppendThreads) {
             double sn, cs;
             sincos((double)(pos0 + i / (HD / 2)) * a.inv_freq[i % (HD / 2)], &sn, &cs);
             turn[i] = make_float2((float)cs, (float)sn);
         }
         __syncthreads();
-        for (int i = tid; i < count * (q1 - q0) * (HD / 2); i += kAppendThreads) {
-            const int d = i % (HD / 2), h = q0 + i / (HD / 2) % (q1 - q0), t = i / (HD / 2) / (q1 - q0);
-            const float2 w = turn[t * (HD / 2) + d];
-            const __half *x = a.q + (size_t)(tok0 + t) * a.q_stride + h * HD + d;
-            __half *y = a.q_out + (size_t)(tok0 + t) * a.q_out_stride + h * HD + d;
-            const float x0 = __half2float(x[0]), x1 = __half2float(x[HD / 2]);
-            y[0] = __float2half_rn(__fsub_rn(__fmul_rn(x0, w.x), __fmul_rn(x1, w.y)));
-            y[HD / 2] = __float2half_rn(__fadd_rn(__fmul_rn(x1, w.x), __fmul_rn(x0, w.y)));
+        // q: a warp takes a token; its lanes keep their dims and go through the heads
+        for (int t = warp; t < count; t += kAppendThreads / 32) {
+            constexpr int kHeads = 32 / kChunks;             // heads of a step
+            Turn w;
+            w.load(turn + t * (HD / 2) + lane % kChunks * 8);
+            const size_t at = (size_t)(q0 + lane / kChunks) * HD + lane % kChunks * 8;
+            const __half *x = a.q + (size_t)(tok0 + t) * a.q_stride + at;
+            __half *y = a.q_out + (size_t)(tok0 + t) * a.q_out_stride + at;
+            for (int h = lane / kChunks; h < nq; h += kHeads * kAppendUnroll) {
+                uint4 lo[kAppendUnroll], hi[kAppendUnroll];
+#pragma unroll
+                for (int u = 0; u < kAppendUnroll; u++)
+                    if (h + u * kHeads < nq) {
+                        const uint4 *p = reinterpret_cast<const uint4 *>(x + (h - lane / kChunks + u * kHeads) * HD);
+                        lo[u] = p[0];
+                        hi[u] = p[kChunks];
+                    }
+#pragma unroll
+                for (int u = 0; u < kAppendUnroll; u++)
+                    if (h + u * kHeads < nq) {
+                        w.apply(lo[u], hi[u]);
+                        uint4 *p = reinterpret_cast<uint4 *>(y + (h - lane / kChunks + u * kHeads) * HD);
+                        p[0] = lo[u];
+                        p[kChunks] = hi[u];
+                    }
+            }
         }
         for (int h = kv0; h < kv1; h++)
             for (int which = 0; which < 2; which++) {
-                __half *tk = a.tail_k + (size_t)seq * a.tail_k_stride + (size_t)h * b * HD;
-                __half *tv = a.tail_v + (size_t)seq * a.tail_v_stride + (size_t)h * b * HD;
+                __half *tail = (which == 0 ? a.tail_k + (size_t)seq * a.tail_k_stride : a.tail_v + (size_t)seq * a.tail_v_stride) + (size_t)h * b * HD;
                 __syncthreads();
-                if (tid == 0) s_amax = 0;
+                if (tid == 0) s_amax[which] = 0;
+                unsigned top = 0;                            // the largest magnitude as bits: an infinity or NaN is above every number
+                auto see = [&](const uint4 &v) {
+                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+                };
                 if (which == 0) {
-                    for (int i = tid; i < count * (HD / 2); i += kAppendThreads) {
-                        const int d = i % (HD / 2), t = i / (HD / 2);
-                        const float2 w = turn[i];
-                        const __half *x = a.k + (size_t)(tok0 + t) * a.k_stride + h * HD + d;
-                        const float x0 = __half2float(x[0]), x1 = __half2float(x[HD / 2]);
-                        tile[(o + t) * HD + d] = __float2half_rn(__fsub_rn(__fmul_rn(x0, w.x), __fmul_rn(x1, w.y)));
-                        tile[(o + t) * HD + d + HD / 2] = __float2half_rn(__fadd_rn(__fmul_rn(x1, w.x), __fmul_rn(x0, w.y)));
+                    for (int i = tid; i < count * kChunks; i += kAppendThreads) {
+                        const int t = i / kChunks, d = i % kChunks * 8;
+                        const uint4 *p = reinterpret_cast<const uint4 *>(a.k + (size_t)(tok0 + t) * a.k_stride + h * HD + d);
+                        uint4 lo = p[0], hi = p[kChunks];
+                        Turn w;
+                        w.load(turn + t * (HD / 2) + d);
+                        w.apply(lo, hi);
+                        see(lo);
+                        see(hi);
+                        uint4 *to = reinterpret_cast<uint4 *>(id < 0 ? tail + (o + t) * HD + d : tile + (o + t) * HD + d);
+                        to[0] = lo;
+                        to[kChunks] = hi;
                     }
                 } else {
-                    for (int i = tid; i < count * HD; i += kAppendThreads)
-                        tile[(o + i / HD) * HD + i % HD] = a.v[(size_t)(tok0 + i / HD) * a.v_stride + h * HD + i % HD];
-                }
-                if (id < 0) {
-                    __syncthreads();
-                    for (int i = tid; i < count * HD; i += kAppendThreads) {
-                        const int t = o + i / HD, d = i % HD;
-                        if (which == 0) tk[t * HD + d] = tile[t * HD + d];
-                        else tv[((t >> 1) * HD + d) * 2 + (t & 1)] = tile[t * HD + d];
+                    for (int i = tid; i < count * (HD / 8); i += kAppendThreads) {
+                        const int t = i / (HD / 8), d = i % (HD / 8) * 8;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(a.v + (size_t)(tok0 + t) * a.v_stride + h * HD + d);
+                        see(v);
+                        if (id >= 0) *reinterpret_cast<uint4 *>(tile + (o + t) * HD + d) = v;
+                        else {
+                            const __half *e = reinterpret_cast<const __half *>(&v);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) tail[((o + t) >> 1) * (2 * HD) + (d + j) * 2 + ((o + t) & 1)] = e[j];
+                        }
                     }
-                    continue;
                 }
-                for (int i = tid; i < o * HD; i += kAppendThreads) {
-                    const int t = i / HD, d = i % HD;
-                    tile[i] = which == 0 ? tk[i] : tv[((t >> 1) * HD + d) * 2 + (t & 1)];
+                if (id < 0) continue;
+                for (int i = tid; i < o * (HD / 8); i += kAppendThreads) {
+                    const int t = i / (HD / 8), d = i % (HD / 8) * 8;
+                    uint4 v;
+                    if (which == 0) v = *reinterpret_cast<const uint4 *>(tail + t * HD + d);
+                    else {
+                        __half *e = reinterpret_cast<__half *>(&v);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) e[j] = tail[(t >> 1) * (2 * HD) + (d + j) * 2 + (t & 1)];
+                    }
+                    see(v);
+                    *reinterpret_cast<uint4 *>(tile + t * HD + d) = v;
                 }
                 __syncthreads();
-                // the largest magnitude as bits: an infinity or NaN is larger than every number
-                unsigned m = 0;
-                for (int i = tid; i < b * HD; i += kAppendThreads) m = max(m, (unsigned)(__half_as_ushort(tile[i]) & 0x7FFF));
-                m = __reduce_max_sync(kFullMask, m);
-                if ((tid & 31) == 0) atomicMax(&s_amax, m);
+                top = __reduce_max_sync(kFullMask, max(top & 0xFFFFu, top >> 16));
+                if (lane == 0) atomicMax(&s_amax[which], top);
                 __syncthreads();
-                const bool finite = s_amax < 0x7C00;
-                const float amax = fmaxf(__half2float(__ushort_as_half((unsigned short)s_amax)), kTinyAmax), top = KIND == kKvInt8 ? 127.f : 448.f;
-                const float inv = __fdiv_rn(top, amax);
-                uint8_t *out = a.data + ((size_t)id * a.n_kv + h) * (size_t)(2 * b * HD);
-                for (int i = tid; i < b * HD; i += kAppendThreads) {
-                    const int t = i / HD, d = i % HD;
-                    const float x = __fmul_rn(__half2float(tile[i]), inv);
-                    uint8_t c;
-                    if constexpr (KIND == kKvInt8) c = (uint8_t)(finite ? (int)rintf(x) + 128 : 128);
-                    else c = finite ? (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3) : 0;
-                    out[((t >> 4) * 2 + which) * (16 * HD) + (which == 0 ? k_byte(t & 15, d, HD) : v_byte(t & 15, d, HD))] = c;
+                const unsigned bits = s_amax[which];
+                const bool finite = bits < 0x7C00;
+                const float amax = fmaxf(__half2float(__ushort_as_half((unsigned short)bits)), kTinyAmax), full = KIND == kKvInt8 ? 127.f : 448.f;
+                const float inv = __fdiv_rn(full, amax);
+                uint8_t *out = a.data + ((size_t)id * a.n_kv + h) * (size_t)(2 * b * HD) + which * (16 * HD);
+                for (int i = tid; i < b * HD / 16; i += kAppendThreads) {
+                    // 16 bytes of a unit
+                    const int u = i / HD, at = i % HD * 16;
+                    uint32_t word[4];
+                    if (which == 0) {                        // (group of 8 tokens, half of 64 dims, token, dim)
+                        const int t = (at >> 9) / (HD >> 6) * 8 + ((at >> 6) & 7), d = (at >> 9) % (HD >> 6) * 64 + (at & 63);
+                        const __half2 *src = reinterpret_cast<const __half2 *>(tile + (16 * u + t) * HD + d);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float2 x = __half22float2(src[2 * k]), y = __half22float2(src[2 * k + 1]);
+                            word[k] = code_of<KIND>(__fmul_rn(x.x, inv), finite) | code_of<KIND>(__fmul_rn(x.y, inv), finite) << 8 |
+                                      code_of<KIND>(__fmul_rn(y.x, inv), finite) << 16 | code_of<KIND>(__fmul_rn(y.y, inv), finite) << 24;
+                        }
+                    } else {                                 // token 8h + 2c + e, dim g * HD/8 + 4n + j, order (n, g, c, j, h, e)
+                        const int c = (at >> 4) & 3, g = (at >> 6) & 7, n = at >> 9;
+                        const __half *src = tile + (16 * u + 2 * c) * HD + g * (HD / 8) + 4 * n;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            word[j] = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                word[j] |= code_of<KIND>(__fmul_rn(__half2float(src[((k >> 1) * 8 + (k & 1)) * HD + j]), inv), finite) << (8 * k);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(out + (size_t)u * (32 * HD) + at) = make_uint4(word[0], word[1], word[2], word[3]);
                 }
                 // a block that holds something not finite stands for NaN everywhere
-                if (tid == 0) reinterpret_cast<float *>(a.scales + (size_t)id * a.n_kv + h)[which] = finite ? __fmul_rn(amax, 1.f / top) : NAN;
+                if (tid == 0) reinterpret_cast<float *>(a.scales + (size_t)id * a.n_kv + h)[which] = finite ? __fmul_rn(amax, 1.f / full) : NAN;
             }
-        if (part == 1 || extra < 0 || extra >= *a.n_runs) return;
+        if (part == 1 || extra < 0 || extra >= n_runs) return;
         run = extra;
     }
+}
+
+template <typename... Args>
+int launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return check_launch();
 }
 
 }  // namespace
@@ -275,9 +389,8 @@ extern "C" int qtip_kv_plan(int *tables, const int *lengths, const int *new_toke
     if (!aligned(runs, 16)) return QTIP_ERR_ALIGNMENT;
     const PlanArgs a = {tables, lengths, new_tokens, lengths_out, runs, n_runs, n_seqs, max_blocks, n_blocks, block, n_tokens, status};
     const size_t smem = (size_t)((n_blocks + 31) / 32) * 4;
-    QTIP_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanMaxBlocks + 31) / 32 * 4));
-    kv_plan_kernel<<<1, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-    return check_launch();
+    if (smem > 16384) QTIP_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanMaxBlocks + 31) / 32 * 4));
+    return launch_dependent(kv_plan_kernel, dim3(1), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), a);
 }
 
 extern "C" int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const void *q, long q_stride, const void *k, long k_stride, const void *v,
@@ -298,7 +411,9 @@ extern "C" int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const v
     const size_t smem = (size_t)block * head_dim * (sizeof(float) + sizeof(__half));
     auto kernel = head_dim == 128 ? (kind == kKvInt8 ? append_kernel<128, kKvInt8> : append_kernel<128, kKvE4m3>)
                                   : (kind == kKvInt8 ? append_kernel<64, kKvInt8> : append_kernel<64, kKvE4m3>);
-    QTIP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 128 * 6));
-    kernel<<<dim3(max_runs, min(n_kv_heads, 8)), kAppendThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-    return check_launch();
+    if (smem > 48 * 1024 - 64) QTIP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 128 * 6));
+    // shares of the heads: four CTAs per SM, where there are as many heads
+    const int wanted = (4 * sm_count() + max_runs - 1) / max_runs, shares = wanted < 1 ? 1 : wanted < n_kv_heads ? wanted : n_kv_heads;
+    const int per = (n_kv_heads + shares - 1) / shares;
+    return launch_dependent(kernel, dim3(max_runs, (n_kv_heads + per - 1) / per), dim3(kAppendThreads), smem, static_cast<cudaStream_t>(stream), a);
 }

@@ -425,7 +425,8 @@ int qtip_attn_decode_batch(void *out, const void *q, const void *cache_k, const 
  * QTIP_KV_INT8: value = (byte - 128) * scale, scale = largest magnitude / 127; QTIP_KV_E4M3: value = e4m3 * scale, scale = largest / 448
  * (the largest is at least 2^-24).  A block in which some value is not finite has the scale NaN: all its tokens stand for NaN.
  * head_dim 64 or 128.  All follow stream order for every operand.  `status` (optional) as for the decode loop, and 8: the pool is exhausted,
- * 16: a table names no block of the pool, 32: a beam's parent outside its group.
+ * 16: a table names no block of the pool (attention: the sequence's result is NaN), 32: a beam's parent outside its group, 64: a bounded wait of
+ * the attention for its own copies ran out (results are meaningless, the kernel ends).
  * ------------------------------------------------------------------------------------------ */
 enum { QTIP_KV_INT8 = 0, QTIP_KV_E4M3 = 1 };
 

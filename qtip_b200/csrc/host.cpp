@@ -11,6 +11,8 @@
 //                  kernel_layout, rcp, tp, workspace|None) -> (output, launches)
 //   matvec_workspace(device_index, m, n, bs) -> uint8 tensor    the fused matvec's scratch of (device, current stream)
 //   gemm_status(device_index) -> int32 tensor                   the decompress-GEMM's status word of a device
+//   kv_plan, rope_kv_append_paged, attn_decode_paged, beam_select, beam_reorder: the checks and launches of the functions of the same
+//   names in ops.py (calls of 3 to 8 us of GPU work, for which the checks in Python took 13 to 25 us) -> launches
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -310,10 +312,235 @@ PyObject *py_gemm_status(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     });
 }
 
+// ---- batched decoding over the 8-bit cache, and beam search: checks and launches -----------------------------------------------------------
+const at::Tensor *maybe(PyObject *o, const char *name) {
+    if (o == Py_None) return nullptr;
+    if (!THPVariable_Check(o)) throw Failure{std::string(name) + " must be a tensor"};
+    return &THPVariable_Unpack(o);
+}
+const at::Tensor &given(PyObject *o, const char *name) {
+    const at::Tensor *t = maybe(o, name);
+    if (!t) throw Failure{std::string(name) + " must be a tensor"};
+    return *t;
+}
+// The call goes to the current device and stream (so that a step can be captured): tensors that live elsewhere are refused.
+void here(std::initializer_list<const at::Tensor *> tensors) {
+    for (const at::Tensor *t : tensors)
+        if (t && !t->is_cuda()) throw Failure{"qtip_b200 runs on CUDA tensors only (no CPU fallback)"};
+    const int cur = c10::cuda::current_device();
+    for (const at::Tensor *t : tensors)
+        if (t && t->get_device() != cur)
+            throw Failure{"tensor on cuda:" + std::to_string(t->get_device()) + " but the current device is cuda:" + std::to_string(cur) +
+                          ": call torch.cuda.set_device() / use torch.cuda.device() around qtip_b200 launches"};
+}
+std::string text(at::IntArrayRef shape) {
+    std::string s = "(";
+    for (size_t i = 0; i < shape.size(); i++) s += (i ? ", " : "") + std::to_string(shape[i]);
+    return s + ")";
+}
+void expect(const char *name, const at::Tensor &t, at::ScalarType type, at::IntArrayRef shape, bool contiguous = true) {
+    if (t.scalar_type() != type) throw Failure{std::string(name) + ": " + c10::toString(type) + " expected, not " + c10::toString(t.scalar_type())};
+    if (t.sizes() != shape) throw Failure{std::string(name) + ": shape " + text(shape) + " expected, not " + text(t.sizes())};
+    if (contiguous && !t.is_contiguous()) throw Failure{std::string(name) + " has to be contiguous"};
+}
+// Row stride of a (rows, width) fp16 matrix whose rows are contiguous.
+long rows_of(const char *name, const at::Tensor &t, int64_t rows, int64_t width) {
+    if (t.dim() != 2 || t.scalar_type() != at::kHalf || t.size(0) != rows || t.size(1) != width)
+        throw Failure{std::string(name) + ": " + text({rows, width}) + " fp16 expected, not " + text(t.sizes()) + " " + c10::toString(t.scalar_type())};
+    if (width > 1 && t.stride(1) != 1) throw Failure{std::string(name) + ": the values of a row have to be contiguous"};
+    return rows > 1 ? t.stride(0) : width;
+}
+void *current_stream() { return at::cuda::getCurrentCUDAStream(c10::cuda::current_device()).stream(); }
+unsigned *status_of(const at::Tensor *t) {
+    if (!t) return nullptr;
+    if (t->nbytes() < 4 || t->element_size() != 4) throw Failure{"status: a 32-bit word expected"};
+    return static_cast<unsigned *>(t->data_ptr());
+}
+
+struct KvCache {
+    const at::Tensor &data, &scales, &tail_k, &tail_v;
+    int64_t blocks, kv, block, hd, seqs;
+    KvCache(PyObject *d, PyObject *s, PyObject *k, PyObject *v)
+        : data(given(d, "data")), scales(given(s, "scales")), tail_k(given(k, "tail_k")), tail_v(given(v, "tail_v")) {
+        if (data.dim() != 5 || data.size(3) != 2 || data.size(4) % 16 || tail_k.dim() != 4)
+            throw Failure{"data: (n_blocks, n_kv, block/16, 2, 16*head_dim) uint8 and tail_k: (n_seqs, n_kv, block, head_dim) fp16 expected"};
+        blocks = data.size(0); kv = data.size(1); block = data.size(2) * 16; hd = data.size(4) / 16; seqs = tail_k.size(0);
+        expect("data", data, at::kByte, data.sizes());
+        expect("scales", scales, at::kFloat, {blocks, kv, 4});
+        expect("tail_k", tail_k, at::kHalf, {seqs, kv, block, hd}, false);
+        expect("tail_v", tail_v, at::kHalf, {seqs, kv, block / 2, hd, 2}, false);
+        if (hd == 0 || blocks == 0 || seqs == 0 || kv == 0) throw Failure{"an empty cache"};
+        // one sequence's part is contiguous
+        if (tail_k.stride(3) != 1 || tail_k.stride(2) != hd || (kv > 1 && tail_k.stride(1) != block * hd) || tail_v.stride(4) != 1 || tail_v.stride(3) != 2 ||
+            (block > 2 && tail_v.stride(2) != 2 * hd) || (kv > 1 && tail_v.stride(1) != block * hd))
+            throw Failure{"the tails of one sequence have to be contiguous"};
+        if (seqs > 1 && (tail_k.stride(0) < kv * block * hd || tail_v.stride(0) < kv * block * hd)) throw Failure{"the tails of two sequences overlap"};
+    }
+    long stride_k() const { return seqs > 1 ? tail_k.stride(0) : 0; }
+    long stride_v() const { return seqs > 1 ? tail_v.stride(0) : 0; }
+    const at::Tensor *list[4] = {&data, &scales, &tail_k, &tail_v};
+};
+
+template <class F>
+PyObject *launching(Py_ssize_t nargs, Py_ssize_t want, const char *name, F body) {
+    return guarded([&]() -> PyObject * {
+        if (nargs != want) throw Failure{std::string(name) + " takes " + std::to_string(want) + " arguments"};
+        return PyLong_FromLong(body());
+    });
+}
+
+PyObject *py_kv_plan(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return launching(nargs, 10, "kv_plan", [&] {
+        const at::Tensor &tables = given(a[0], "tables"), &lengths = given(a[1], "lengths"), &fresh = given(a[2], "new"),
+                         &lengths_out = given(a[3], "lengths_out"), &runs = given(a[4], "runs"), &n_runs = given(a[5], "n_runs"),
+                         *status = maybe(a[9], "status");
+        const long n_blocks = int_arg(a[6]), block = int_arg(a[7]), n_tokens = int_arg(a[8]);
+        here({&tables, &lengths, &fresh, &lengths_out, &runs, &n_runs, status});
+        if (tables.dim() != 2 || runs.dim() != 2) throw Failure{"tables: (n_seqs, max_blocks), runs: (max_runs, 8) expected"};
+        const int64_t S = tables.size(0);
+        expect("tables", tables, at::kInt, {S, tables.size(1)});
+        expect("lengths", lengths, at::kInt, {S});
+        expect("new", fresh, at::kInt, {S});
+        expect("lengths_out", lengths_out, at::kInt, {S});
+        expect("runs", runs, at::kInt, {runs.size(0), 8});
+        expect("n_runs", n_runs, at::kInt, {1});
+        if (n_blocks > INT32_MAX || n_tokens > INT32_MAX || block > INT32_MAX) throw Failure{"n_blocks, block, n_tokens: 32-bit numbers expected"};
+        check(qtip_kv_plan(static_cast<int *>(tables.data_ptr()), static_cast<const int *>(lengths.data_ptr()), static_cast<const int *>(fresh.data_ptr()),
+                           static_cast<int *>(lengths_out.data_ptr()), static_cast<int *>(runs.data_ptr()), static_cast<int *>(n_runs.data_ptr()), (int)S,
+                           (int)tables.size(1), (int)n_blocks, (int)block, (int)n_tokens, (int)std::min<int64_t>(runs.size(0), INT32_MAX), status_of(status),
+                           current_stream()),
+              "qtip_kv_plan");
+        return 1L;
+    });
+}
+
+PyObject *py_rope_kv_append_paged(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return launching(nargs, 13, "rope_kv_append_paged", [&] {
+        const at::Tensor &q_out = given(a[0], "q_out"), &q = given(a[1], "q"), &k = given(a[2], "k"), &v = given(a[3], "v");
+        const KvCache c(a[4], a[5], a[6], a[7]);
+        const at::Tensor &runs = given(a[8], "runs"), &n_runs = given(a[9], "n_runs"), &inv_freq = given(a[10], "inv_freq"), *status = maybe(a[12], "status");
+        here({&q_out, &q, &k, &v, c.list[0], c.list[1], c.list[2], c.list[3], &runs, &n_runs, &inv_freq, status});
+        if (q.dim() != 2 || runs.dim() != 2) throw Failure{"q: (n_tokens, n_heads*head_dim), runs: (max_runs, 8) expected"};
+        const int64_t T = q.size(0), width = q.size(1);
+        expect("runs", runs, at::kInt, {runs.size(0), 8});
+        expect("n_runs", n_runs, at::kInt, {1});
+        expect("inv_freq", inv_freq, at::kDouble, {c.hd / 2});
+        if (width % c.hd) throw Failure{"q: a multiple of head_dim values in a row expected"};
+        const long sqo = rows_of("q_out", q_out, T, width), sq = rows_of("q", q, T, width), sk = rows_of("k", k, T, c.kv * c.hd), sv = rows_of("v", v, T, c.kv * c.hd);
+        if (T > INT32_MAX || c.blocks > INT32_MAX) throw Failure{"too many token rows or blocks"};
+        check(qtip_rope_kv_append_paged(q_out.data_ptr(), sqo, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, c.data.data_ptr(),
+                                        static_cast<float *>(c.scales.data_ptr()), c.tail_k.data_ptr(), c.stride_k(), c.tail_v.data_ptr(), c.stride_v(),
+                                        static_cast<const int *>(runs.data_ptr()), static_cast<const int *>(n_runs.data_ptr()),
+                                        (int)std::min<int64_t>(runs.size(0), INT32_MAX), static_cast<const double *>(inv_freq.data_ptr()), (int)T,
+                                        (int)c.seqs, (int)(width / c.hd), (int)c.kv, (int)c.hd, (int)c.blocks, (int)c.block, (int)int_arg(a[11]),
+                                        status_of(status), current_stream()),
+              "qtip_rope_kv_append_paged");
+        return 1L;
+    });
+}
+
+PyObject *py_attn_decode_paged(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return launching(nargs, 11, "attn_decode_paged", [&] {
+        const at::Tensor &out = given(a[0], "out"), &q = given(a[1], "q");
+        const KvCache c(a[2], a[3], a[4], a[5]);
+        const at::Tensor &tables = given(a[6], "tables"), &lengths = given(a[7], "lengths"), *workspace = maybe(a[9], "workspace"),
+                         *status = maybe(a[10], "status");
+        here({&out, &q, c.list[0], c.list[1], c.list[2], c.list[3], &tables, &lengths, workspace, status});
+        if (q.dim() != 2 || tables.dim() != 2 || q.size(1) % c.hd) throw Failure{"q: (n_seqs, n_heads*head_dim), tables: (n_seqs, max_blocks) expected"};
+        const int64_t width = q.size(1), n_heads = width / c.hd;
+        expect("tables", tables, at::kInt, {c.seqs, tables.size(1)});
+        expect("lengths", lengths, at::kInt, {c.seqs});
+        const long so = rows_of("out", out, c.seqs, width), sq = rows_of("q", q, c.seqs, width);
+        if (n_heads > INT32_MAX || c.blocks > INT32_MAX || tables.size(1) > INT32_MAX) throw Failure{"too many heads or blocks"};
+        at::Tensor own;                  // from torch's allocator: of the stream, or of the graph that is being captured
+        if (!workspace) {
+            const size_t need = qtip_attn_paged_workspace_bytes((int)c.seqs, (int)n_heads, (int)c.kv, (int)c.hd);
+            own = at::empty({(int64_t)std::max<size_t>(need, 1)}, q.options().dtype(at::kByte));
+            workspace = &own;
+        }
+        check(qtip_attn_decode_paged(out.data_ptr(), so, q.data_ptr(), sq, c.data.data_ptr(), static_cast<const float *>(c.scales.data_ptr()),
+                                     c.tail_k.data_ptr(), c.stride_k(), c.tail_v.data_ptr(), c.stride_v(), static_cast<const int *>(tables.data_ptr()),
+                                     static_cast<const int *>(lengths.data_ptr()), (int)c.seqs, (int)n_heads, (int)c.kv, (int)c.hd, (int)tables.size(1),
+                                     (int)c.blocks, (int)c.block, (int)int_arg(a[8]), workspace->data_ptr(), workspace->nbytes(), status_of(status),
+                                     current_stream()),
+              "qtip_attn_decode_paged");
+        return 1L;
+    });
+}
+
+PyObject *py_beam_select(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return launching(nargs, 8, "beam_select", [&] {
+        const at::Tensor &tokens = given(a[0], "tokens"), &parents = given(a[1], "parents"), &scores = given(a[2], "scores"), &logits = given(a[3], "logits"),
+                         &prev_scores = given(a[4], "prev_scores"), *prev_tokens = maybe(a[5], "prev_tokens"), *status = maybe(a[7], "status");
+        here({&tokens, &parents, &scores, &logits, &prev_scores, prev_tokens, status});
+        if (tokens.dim() != 2 || logits.dim() != 2) throw Failure{"tokens: (groups, width), logits: (groups * width, vocab) expected"};
+        const int64_t G = tokens.size(0), W = tokens.size(1), vocab = logits.size(1);
+        expect("tokens", tokens, at::kLong, {G, W});
+        expect("parents", parents, at::kInt, {G, W});
+        expect("scores", scores, at::kFloat, {G, W});
+        expect("prev_scores", prev_scores, at::kFloat, {G, W});
+        if (prev_tokens) expect("prev_tokens", *prev_tokens, at::kLong, {G, W});
+        if (logits.size(0) != G * W || (vocab > 1 && logits.stride(1) != 1)) throw Failure{"logits: (groups * width, vocab) with contiguous rows expected, not " + text(logits.sizes())};
+        const long long eos = PyLong_AsLongLong(a[6]);
+        if (eos == -1 && PyErr_Occurred()) throw Failure{""};
+        if (vocab > INT32_MAX) throw Failure{"too large a vocabulary"};
+        check(qtip_beam_select(reinterpret_cast<long long *>(tokens.data_ptr()), static_cast<int *>(parents.data_ptr()), static_cast<float *>(scores.data_ptr()),
+                               logits.data_ptr(), dtype_id(logits), G * W > 1 ? logits.stride(0) : vocab, static_cast<const float *>(prev_scores.data_ptr()),
+                               prev_tokens ? reinterpret_cast<const long long *>(prev_tokens->data_ptr()) : nullptr, (int)G, (int)W, (int)vocab, eos,
+                               status_of(status), current_stream()),
+              "qtip_beam_select");
+        return 1L;
+    });
+}
+
+PyObject *py_beam_reorder(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    return launching(nargs, 4, "beam_reorder", [&] {
+        const at::Tensor &parents = given(a[1], "parents"), *lengths = maybe(a[2], "lengths"), *status = maybe(a[3], "status");
+        here({&parents, lengths, status});
+        if (parents.dim() != 2) throw Failure{"parents: (groups, width) expected"};
+        const int64_t G = parents.size(0), W = parents.size(1);
+        expect("parents", parents, at::kInt, {G, W});
+        if (lengths) expect("lengths", *lengths, at::kInt, {G * W});
+        if (!PyList_Check(a[0]) && !PyTuple_Check(a[0])) throw Failure{"states: a list of (tensor, tokens per row, modulus) expected"};
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(a[0]);
+        if (n < 1 || n > 8) throw Failure{"1 to 8 states expected, not " + std::to_string(n)};
+        qtip_beam_state list[8];
+        for (Py_ssize_t i = 0; i < n; i++) {
+            PyObject *s = PySequence_Fast_GET_ITEM(a[0], i);
+            if (!PyTuple_Check(s) || PyTuple_GET_SIZE(s) != 3) throw Failure{"a state is (tensor, tokens per row, modulus)"};
+            const at::Tensor &t = given(PyTuple_GET_ITEM(s, 0), "a state's tensor");
+            here({&t});
+            const long per_row = int_arg(PyTuple_GET_ITEM(s, 1)), mod = int_arg(PyTuple_GET_ITEM(s, 2));
+            if (t.dim() != 4 || t.size(0) != G * W || t.numel() == 0) throw Failure{"a state is (" + std::to_string(G * W) + ", outer, rows, values), not " + text(t.sizes())};
+            if ((t.size(3) > 1 && t.stride(3) != 1) || (t.size(2) > 1 && t.stride(2) != t.size(3))) throw Failure{"the rows of a state have to be contiguous"};
+            const long size = (long)t.element_size(), piece = t.size(2) * t.size(3) * size;
+            if (per_row < 1 || per_row > INT32_MAX || mod < 0 || mod > INT32_MAX || t.size(1) > INT32_MAX || t.size(2) > INT32_MAX || t.size(3) * size > INT32_MAX)
+                throw Failure{"a state's tokens per row, modulus or sizes are out of range"};
+            list[i].base = t.data_ptr();
+            list[i].outer_stride = t.size(1) > 1 ? t.stride(1) * size : piece;
+            list[i].seq_stride = G * W > 1 ? t.stride(0) * size : list[i].outer_stride * t.size(1);
+            list[i].outer = (int)t.size(1);
+            list[i].rows = (int)t.size(2);
+            list[i].row_bytes = (int)(t.size(3) * size);
+            list[i].per_row = (int)per_row;
+            list[i].mod = (int)mod;
+        }
+        check(qtip_beam_reorder(list, (int)n, static_cast<const int *>(parents.data_ptr()), lengths ? static_cast<const int *>(lengths->data_ptr()) : nullptr,
+                                (int)G, (int)W, status_of(status), current_stream()),
+              "qtip_beam_reorder");
+        return 1L;
+    });
+}
+
 PyMethodDef kMethods[] = {
     {"linear_forward", (PyCFunction)(void *)py_linear_forward, METH_FASTCALL, "one QTIP linear on the current stream"},
     {"matvec_workspace", (PyCFunction)(void *)py_matvec_workspace, METH_FASTCALL, "scratch of the fused matvec"},
     {"gemm_status", (PyCFunction)(void *)py_gemm_status, METH_FASTCALL, "status word of the decompress-GEMM"},
+    {"kv_plan", (PyCFunction)(void *)py_kv_plan, METH_FASTCALL, "where new tokens of a batch go"},
+    {"rope_kv_append_paged", (PyCFunction)(void *)py_rope_kv_append_paged, METH_FASTCALL, "rotary embedding and append to the 8-bit cache"},
+    {"attn_decode_paged", (PyCFunction)(void *)py_attn_decode_paged, METH_FASTCALL, "attention over the 8-bit cache"},
+    {"beam_select", (PyCFunction)(void *)py_beam_select, METH_FASTCALL, "the best continuations of groups of beams"},
+    {"beam_reorder", (PyCFunction)(void *)py_beam_reorder, METH_FASTCALL, "states follow their beams"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "native host path of qtip_b200", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

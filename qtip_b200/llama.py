@@ -400,11 +400,13 @@ class QtipLlama:
                          status=self.status)
 
     # -- batched decode: B sequences in lockstep ------------------------------------------------------
-    def enable_batch(self, B):
+    def enable_batch(self, B, kv=None, block=32, n_blocks=None):
         """Buffers for decoding B (<= 8) independent sequences per step (step_batch).  The batch rides in the matvec
         launches (the packed matrices are streamed once for all B rows); the transforms run as row-batched launches of
         the transform kernel, rotary embedding, attention and sampling as one launch for all sequences.  Works for every shape and for
-        tensor parallelism (NCCL all-reduce after o_proj and down_proj)."""
+        tensor parallelism (NCCL all-reduce after o_proj and down_proj).
+        kv: None, a key/value cache in fp16 for max_positions of every sequence; "int8" or "e4m3", a pool of n_blocks blocks of `block` tokens in 8
+        bits, which sequences take as they grow (default: enough for all of them)."""
         assert 1 <= B <= ops.MAX_MATVEC_BATCH and not self.fuse_qkv
         s, dev, H, KV, MLP = self.shape, self.device, self.H, self.KV, self.MLP
         f16 = dict(dtype=torch.float16, device=dev)
@@ -419,8 +421,25 @@ class QtipLlama:
         self.b_q, self.b_k, self.b_v = torch.zeros(B, H, **f16), torch.zeros(B, KV, **f16), torch.zeros(B, KV, **f16)
         self.b_attn = torch.zeros(B, H, **f16)
         self.b_g, self.b_u = torch.zeros(B, MLP, **f16), torch.zeros(B, MLP, **f16)
-        self.b_cache_k = torch.zeros(B, s.n_layers, self.max_positions, KV, **f16)
-        self.b_cache_v = torch.zeros_like(self.b_cache_k)
+        self.b_kv = kv
+        if kv is None:
+            self.b_cache_k = torch.zeros(B, s.n_layers, self.max_positions, KV, **f16)
+            self.b_cache_v = torch.zeros_like(self.b_cache_k)
+        else:
+            assert kv in ops.KV_KINDS and block in ops.KV_BLOCKS
+            heads, hd, per_seq = self.n_kv_heads, s.head_dim, max(self.max_positions // block, 1)
+            self.kv_block, self.kv_blocks = block, B * per_seq if n_blocks is None else n_blocks
+            self.kv_data = torch.zeros(s.n_layers, self.kv_blocks, heads, block // 16, 2, 16 * hd, dtype=torch.uint8, device=dev)
+            self.kv_scales = torch.zeros(s.n_layers, self.kv_blocks, heads, 4, **f32)
+            self.kv_tail_k = torch.zeros(B, s.n_layers, heads, block, hd, **f16)
+            self.kv_tail_v = torch.zeros(B, s.n_layers, heads, block // 2, hd, 2, **f16)
+            i32 = dict(dtype=torch.int32, device=dev)
+            self.kv_tables = torch.full((B, per_seq), -1, **i32)
+            self.kv_new, self.kv_lengths = torch.ones(B, **i32), torch.zeros(B, **i32)
+            self.kv_runs, self.kv_n_runs = torch.zeros(ops.kv_runs_capacity(B, B, block), 8, **i32), torch.zeros(1, **i32)
+            self.kv_inv_freq = s.rope_theta ** (-torch.arange(0, hd, 2, dtype=torch.float64, device=dev) / hd)
+            self.kv_workspace = ops.attn_paged_workspace(B, self.n_heads, heads, hd, dev)
+        self.beam_width = 0
         self.b_logits = torch.zeros(B, s.vocab, **f32)
         self.b_out_tokens = torch.zeros(B, self.max_positions + 1, dtype=torch.int64, device=dev)
         need = max(ops._lib.load().qtip_matvec_workspace_bytes(m, n, B)
@@ -442,23 +461,37 @@ class QtipLlama:
             self._all_reduce(y)
         ops.rht_fused(y, B, m, out, sign_out=lin.SV32, hadk_bits=self.bits[kf_out], kfac=kf_out, scale=1 / math.sqrt(m))
 
-    def step_batch(self):
-        """One decode step of B sequences on the static batch buffers: b_token -> next tokens, b_pos += 1."""
-        s, B = self.shape, self.B
+    def _attention_batch(self, li):
+        """Rotary embedding, append and attention of one layer for the batch: b_q, b_k, b_v -> b_attn."""
+        s = self.shape
+        if self.b_kv is None:
+            ck, cv = self.b_cache_k[:, li], self.b_cache_v[:, li]
+            ops.rope_kv_append_batch(self.b_q, self.b_k, self.b_v, ck, cv, self.b_pos, self.n_heads, self.n_kv_heads, s.head_dim,
+                                     s.rope_theta, status=self.status)
+            ops.attn_decode_batch(self.b_attn, self.b_q, ck, cv, self.b_pos, self.n_heads, self.n_kv_heads, s.head_dim,
+                                  status=self.status)
+            return
+        cache = self.kv_data[li], self.kv_scales[li], self.kv_tail_k[:, li], self.kv_tail_v[:, li]
+        ops.rope_kv_append_paged(self.b_q, self.b_q, self.b_k, self.b_v, *cache, self.kv_runs, self.kv_n_runs, self.kv_inv_freq, self.b_kv,
+                                 status=self.status)
+        ops.attn_decode_paged(self.b_attn, self.b_q, *cache, self.kv_tables, self.kv_lengths, self.b_kv, self.kv_workspace, status=self.status)
+
+    def _forward_batch(self):
+        """b_token at positions b_pos -> b_logits; the cache holds the tokens."""
+        s = self.shape
         ra, rb = self.b_res
         torch.index_select(self.embed, 0, self.b_token, out=ra)
         self.b_delta.zero_()
+        if self.b_kv is not None:
+            ops.kv_plan(self.kv_tables, self.b_pos, self.kv_new, self.kv_lengths, self.kv_runs, self.kv_n_runs, self.kv_blocks, self.kv_block,
+                        self.B, status=self.status)
         for li, L in enumerate(self.layers):
             # res_b = res_a + delta ; h = RMSNorm(res_b) ; q, k, v
             self._b_linear(L["q"], self.b_delta, residual=ra, residual_out=rb, norm=L["ln1"], kf_in=self.kf_h,
                            kf_out=self.kf_hl, out=self.b_q)
             self._b_linear(L["k"], rb, norm=L["ln1"], kf_in=self.kf_h, kf_out=self.kf_kv, out=self.b_k)
             self._b_linear(L["v"], rb, norm=L["ln1"], kf_in=self.kf_h, kf_out=self.kf_kv, out=self.b_v)
-            ck, cv = self.b_cache_k[:, li], self.b_cache_v[:, li]
-            ops.rope_kv_append_batch(self.b_q, self.b_k, self.b_v, ck, cv, self.b_pos, self.n_heads, self.n_kv_heads, s.head_dim,
-                                     s.rope_theta, status=self.status)
-            ops.attn_decode_batch(self.b_attn, self.b_q, ck, cv, self.b_pos, self.n_heads, self.n_kv_heads, s.head_dim,
-                                  status=self.status)
+            self._attention_batch(li)
             self._b_linear(L["o"], self.b_attn, kf_in=self.kf_hl, kf_out=self.kf_h, out=self.b_delta, all_reduce=True)
             # res_a = res_b + delta ; h = RMSNorm(res_a) ; gate, up ; down(silu(gate) * up)
             self._b_linear(L["gate"], self.b_delta, residual=rb, residual_out=ra, norm=L["ln2"], kf_in=self.kf_h,
@@ -470,10 +503,74 @@ class QtipLlama:
         x32 = (ra + self.b_delta).float()
         hn = (x32 * torch.rsqrt(x32.pow(2).mean(-1, keepdim=True) + s.rms_eps)).half() * self.ln_f
         self.b_logits.copy_(torch.matmul(hn, self.lm_head.T))
+
+    def step_batch(self):
+        """One decode step of B sequences on the static batch buffers: b_token -> next tokens, b_pos += 1.  After enable_beams the next tokens are
+        those of the best beams of each group, and rows whose beam is given up become copies of others."""
+        self._forward_batch()
+        if self.beam_width:
+            self._select_beams()
+            return
         ops.sample_top_k_batch(self.b_token, self.b_out_tokens, self.b_pos, self.b_logits, temperature=0.6, top_k=5,
                                seed=self.sample_seed, status=self.status)
 
+    # -- beam search over the rows of the batch ---------------------------------------------------------
+    def enable_beams(self, width, eos=-1):
+        """The B rows of the batch become B / width groups of `width` beams (after enable_batch, before capture_batch).  feed_beams() takes the prompts,
+        generate_batch() continues; then b_scores (groups, width) holds the sums of log probabilities, b_out_tokens the rows' tokens."""
+        assert 1 <= width <= ops.MAX_BEAMS and self.B % width == 0
+        assert self.b_logits.shape[1] >= width, "fewer tokens than beams"
+        G, dev = self.B // width, self.device
+        self.beam_width, self.beam_eos = width, eos
+        self.b_scores = torch.zeros(G, width, dtype=torch.float32, device=dev)
+        self.b_parents = torch.zeros(G, width, dtype=torch.int32, device=dev)
+        self.b_filled = torch.zeros(self.B, dtype=torch.int32, device=dev)
+        log = (self.b_out_tokens.view(self.B, 1, -1, 1), 1, 0)
+        if self.b_kv is None:
+            self.beam_states = [(self.b_cache_k, 1, 0), (self.b_cache_v, 1, 0), log]
+        else:       # complete blocks are shared by name; the tails are the rows' own
+            flat = lambda t: t.view(self.B, -1, t.shape[3], t.shape[4:].numel())  # noqa: E731
+            self.beam_states = [(flat(self.kv_tail_k), 1, self.kv_block), (flat(self.kv_tail_v), 2, self.kv_block),
+                                (self.kv_tables.view(self.B, 1, -1, 1), self.kv_block, 0), log]
+        self.reset_beams()
+
+    def reset_beams(self):
+        """No tokens, and one beam of each group alive: after the first step all of them hold its continuations."""
+        self.b_pos.zero_()
+        self.b_scores.fill_(-math.inf)
+        self.b_scores[:, 0] = 0.0
+        self.steps_done = 0
+
+    def _select_beams(self):
+        W = self.beam_width
+        tokens = self.b_token.view(-1, W)
+        ops.beam_select(tokens, self.b_parents, self.b_scores, self.b_logits, self.b_scores, tokens, self.beam_eos, status=self.status)
+        torch.add(self.b_pos, 1, out=self.b_filled)
+        ops.beam_reorder(self.beam_states, self.b_parents, self.b_filled, status=self.status)
+        self.b_out_tokens.scatter_(1, self.b_filled.long().view(-1, 1), self.b_token.view(-1, 1))
+        self.b_pos.copy_(self.b_filled)
+
+    def feed_beams(self, prompts):
+        """prompts (groups, n) token ids: every beam of a group takes its group's prompt; the last token's step is the first that selects."""
+        n = prompts.shape[1]
+        assert prompts.shape[0] * self.beam_width == self.B and n >= 1
+        if int(prompts.min()) < 0 or int(prompts.max()) >= self.shape.vocab:
+            raise RuntimeError(f"a token outside the vocabulary of {self.shape.vocab}")
+        self._reserve(n)
+        rows = prompts.to(device=self.device, dtype=torch.int64).repeat_interleave(self.beam_width, 0)
+        for i in range(n):
+            self.b_token.copy_(rows[:, i])
+            self.b_out_tokens[:, i] = rows[:, i]
+            if i + 1 < n:
+                self._forward_batch()
+                self.b_pos.add_(1)
+        (self.b_graph.replay if self.b_graph is not None else self.step_batch)()
+
     def capture_batch(self):
+        """Capture step_batch() into a CUDA graph (two eager warm-up steps first; tokens and positions are restored).  With beams: before the prompts
+        are fed, since the warm-up steps reorder the rows."""
+        if self.beam_width and self.steps_done:
+            raise RuntimeError("capture_batch() with beams comes before feed_beams()")
         tok, pos = self.b_token.clone(), self.b_pos.clone()
         stream = torch.cuda.Stream(device=self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
@@ -490,6 +587,8 @@ class QtipLlama:
                 self.step_batch()
         torch.cuda.current_stream(self.device).wait_stream(stream)
         self.b_token.copy_(tok); self.b_pos.copy_(pos)
+        if self.beam_width:
+            self.reset_beams()
         torch.cuda.synchronize(self.device)
 
     def generate_batch(self, n_tokens):
@@ -549,7 +648,8 @@ class QtipLlama:
         st = int(self.status.item())
         if st:
             raise RuntimeError(f"decode-loop status {st}: 1 = position outside the KV cache, 2 = token outside the "
-                               "embedding table, 4 = token log full")
+                               "embedding table or no continuation, 4 = token log full, 8 = no free block, 16 = a table names no "
+                               "block, 32 = a beam without a parent, 64 = a copy did not arrive")
 
     def feed(self, token_ids):
         """Run the given tokens through the model one position at a time (fills the KV cache); the

@@ -646,26 +646,9 @@ def gemm_plain_supported(m, n, bs):
 
 
 # ---------------------------------------------------------------------------------------------
-# batched decoding over a key/value cache in 8 bits, in blocks of tokens (layout: include/qtip_b200.h)
+# batched decoding over a key/value cache in 8 bits, in blocks of tokens (layout: include/qtip_b200.h).  The arguments are checked in the
+# native host path; all tensors have to be on the current device.
 # ---------------------------------------------------------------------------------------------
-def _expect(name, t, dtype, shape=None, contiguous=True):
-    if t.dtype != dtype:
-        raise RuntimeError(f"{name}: {dtype} expected, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise RuntimeError(f"{name}: shape {tuple(shape)} expected, not {tuple(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise RuntimeError(f"{name} has to be contiguous")
-
-
-def _rows(name, t, width=None):
-    """Row stride of a (rows, width) fp16 matrix whose rows are contiguous."""
-    if t.dim() != 2 or t.dtype != torch.float16 or (width is not None and t.shape[1] != width):
-        raise RuntimeError(f"{name}: (rows, {'width' if width is None else width}) fp16 expected, not {tuple(t.shape)} {t.dtype}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise RuntimeError(f"{name}: the values of a row have to be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def kv_runs_capacity(n_tokens, n_seqs, block):
     """Rows of `runs` that kv_plan needs for n_tokens new tokens of n_seqs sequences."""
     return n_tokens // block + 2 * n_seqs
@@ -674,84 +657,36 @@ def kv_runs_capacity(n_tokens, n_seqs, block):
 def kv_plan(tables, lengths, new, lengths_out, runs, n_runs, n_blocks, block, n_tokens, status=None):
     """qtip_kv_plan: tables (S, max_blocks) int32 (in place), lengths, new, lengths_out (S) int32 -> where the n_tokens rows of new tokens go:
     runs (at least kv_runs_capacity(), 8) and n_runs (1) int32."""
-    _require_cuda(tables, lengths, new, lengths_out, runs, n_runs, status)
-    _check_device(tables, lengths, new, lengths_out, runs, n_runs, status)
-    S = tables.shape[0]
-    _expect("tables", tables, torch.int32, (S, tables.shape[1]))
-    for name, t in (("lengths", lengths), ("new", new), ("lengths_out", lengths_out)):
-        _expect(name, t, torch.int32, (S,))
-    _expect("runs", runs, torch.int32, (runs.shape[0], 8))
-    _expect("n_runs", n_runs, torch.int32)
-    st = _lib.load().qtip_kv_plan(tables.data_ptr(), lengths.data_ptr(), new.data_ptr(), lengths_out.data_ptr(), runs.data_ptr(), n_runs.data_ptr(), S,
-                                  tables.shape[1], n_blocks, block, n_tokens, runs.shape[0], _status_ptr(status), _stream())
-    _lib.check(st, "qtip_kv_plan")
     global launch_count
-    launch_count += 1
+    launch_count += _lib.host().kv_plan(tables, lengths, new, lengths_out, runs, n_runs, n_blocks, block, n_tokens, status)
 
 
-def _kv_cache(data, scales, tail_k, tail_v):
-    """(n_blocks, n_kv, block, hd, n_seqs) of one layer's cache, after checking that its parts agree."""
-    if data.dim() != 5 or data.shape[3] != 2 or data.shape[4] % 16:
-        raise RuntimeError("data: (n_blocks, n_kv, block/16, 2, 16*head_dim) uint8 expected")
-    nb, kv, units, _, w = data.shape
-    block, hd, S = units * 16, w // 16, tail_k.shape[0]
-    _expect("data", data, torch.uint8)
-    _expect("scales", scales, torch.float32, (nb, kv, 4))
-    _expect("tail_k", tail_k, torch.float16, (S, kv, block, hd), contiguous=False)
-    _expect("tail_v", tail_v, torch.float16, (S, kv, block // 2, hd, 2), contiguous=False)
-    if S and not (tail_k[0].is_contiguous() and tail_v[0].is_contiguous()):
-        raise RuntimeError("the tails of one sequence have to be contiguous")
-    return nb, kv, block, hd, S
+def _kv_kind(kind):
+    if kind not in KV_KINDS:
+        raise RuntimeError(f"kind: one of {sorted(KV_KINDS)} expected, not {kind!r}")
+    return KV_KINDS[kind]
 
 
 def rope_kv_append_paged(q_out, q, k, v, data, scales, tail_k, tail_v, runs, n_runs, inv_freq, kind, status=None):
     """qtip_rope_kv_append_paged: q (T, n_heads*hd) rotated into q_out (may be q), k (T, n_kv*hd) rotated and v appended along the runs of kv_plan.
     inv_freq: (hd/2) float64.  kind: "int8" or "e4m3"."""
-    _require_cuda(q_out, q, k, v, data, scales, tail_k, tail_v, runs, n_runs, inv_freq, status)
-    _check_device(q_out, q, k, v, data, scales, tail_k, tail_v, runs, n_runs, inv_freq, status)
-    nb, kv, block, hd, S = _kv_cache(data, scales, tail_k, tail_v)
-    T = q.shape[0]
-    if q.dim() != 2 or q.shape[1] % hd or q_out.shape != q.shape or k.shape[0] != T or v.shape[0] != T:
-        raise RuntimeError("q, q_out (T, n_heads*head_dim), k and v (T, n_kv*head_dim) expected")
-    _expect("runs", runs, torch.int32, (runs.shape[0], 8))
-    _expect("n_runs", n_runs, torch.int32)
-    _expect("inv_freq", inv_freq, torch.float64, (hd // 2,))
-    st = _lib.load().qtip_rope_kv_append_paged(q_out.data_ptr(), _rows("q_out", q_out), q.data_ptr(), _rows("q", q), k.data_ptr(), _rows("k", k, kv * hd),
-                                               v.data_ptr(), _rows("v", v, kv * hd), data.data_ptr(), scales.data_ptr(), tail_k.data_ptr(),
-                                               tail_k.stride(0), tail_v.data_ptr(), tail_v.stride(0), runs.data_ptr(), n_runs.data_ptr(), runs.shape[0],
-                                               inv_freq.data_ptr(), T, S, q.shape[1] // hd, kv, hd, nb, block, KV_KINDS[kind], _status_ptr(status),
-                                               _stream())
-    _lib.check(st, "qtip_rope_kv_append_paged")
     global launch_count
-    launch_count += 1
+    launch_count += _lib.host().rope_kv_append_paged(q_out, q, k, v, data, scales, tail_k, tail_v, runs, n_runs, inv_freq, _kv_kind(kind), status)
     return q_out
 
 
 def attn_paged_workspace(n_seqs, n_heads, n_kv_heads, head_dim, device):
-    """Workspace of attn_decode_paged: for calls that do not overlap."""
-    return torch.empty(_lib.load().qtip_attn_paged_workspace_bytes(n_seqs, n_heads, n_kv_heads, head_dim), dtype=torch.uint8, device=device)
+    """Workspace of attn_decode_paged, for calls that do not overlap."""
+    with torch.cuda.device(device):
+        need = _lib.load().qtip_attn_paged_workspace_bytes(n_seqs, n_heads, n_kv_heads, head_dim)
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
 
 
 def attn_decode_paged(out, q, data, scales, tail_k, tail_v, tables, lengths, kind, workspace=None, status=None):
     """qtip_attn_decode_paged: out, q (S, n_heads*hd) fp16, one new token per sequence, over its lengths[s] cached tokens (0: zeros).  Without a
     workspace the call takes one from torch's allocator."""
-    _require_cuda(out, q, data, scales, tail_k, tail_v, tables, lengths, workspace, status)
-    _check_device(out, q, data, scales, tail_k, tail_v, tables, lengths, workspace, status)
-    nb, kv, block, hd, S = _kv_cache(data, scales, tail_k, tail_v)
-    if q.dim() != 2 or q.shape[0] != S or q.shape[1] % hd or out.shape != q.shape:
-        raise RuntimeError("q, out: (n_seqs, n_heads*head_dim) expected")
-    _expect("tables", tables, torch.int32, (S, tables.shape[1]))
-    _expect("lengths", lengths, torch.int32, (S,))
-    n_heads = q.shape[1] // hd
-    if workspace is None:
-        workspace = attn_paged_workspace(S, n_heads, kv, hd, q.device)
-    st = _lib.load().qtip_attn_decode_paged(out.data_ptr(), _rows("out", out), q.data_ptr(), _rows("q", q), data.data_ptr(), scales.data_ptr(),
-                                            tail_k.data_ptr(), tail_k.stride(0), tail_v.data_ptr(), tail_v.stride(0), tables.data_ptr(),
-                                            lengths.data_ptr(), S, n_heads, kv, hd, tables.shape[1], nb, block, KV_KINDS[kind], workspace.data_ptr(),
-                                            workspace.numel() * workspace.element_size(), _status_ptr(status), _stream())
-    _lib.check(st, "qtip_attn_decode_paged")
     global launch_count
-    launch_count += 1
+    launch_count += _lib.host().attn_decode_paged(out, q, data, scales, tail_k, tail_v, tables, lengths, _kv_kind(kind), workspace, status)
     return out
 
 
@@ -761,47 +696,13 @@ def attn_decode_paged(out, q, data, scales, tail_k, tail_v, tables, lengths, kin
 def beam_select(tokens, parents, scores, logits, prev_scores, prev_tokens=None, eos=-1, status=None):
     """qtip_beam_select: logits (G*W, vocab) fp32 / fp16, prev_scores (G, W) fp32, prev_tokens (G, W) int64 -> tokens (G, W) int64, parents (G, W)
     int32, scores (G, W) fp32.  tokens / scores may be prev_tokens / prev_scores."""
-    _require_cuda(tokens, parents, scores, logits, prev_scores, prev_tokens, status)
-    _check_device(tokens, parents, scores, logits, prev_scores, prev_tokens, status)
-    G, W = tokens.shape
-    _expect("tokens", tokens, torch.int64, (G, W))
-    _expect("parents", parents, torch.int32, (G, W))
-    _expect("scores", scores, torch.float32, (G, W))
-    _expect("prev_scores", prev_scores, torch.float32, (G, W))
-    if prev_tokens is not None:
-        _expect("prev_tokens", prev_tokens, torch.int64, (G, W))
-    if logits.dim() != 2 or logits.shape[0] != G * W or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise RuntimeError(f"logits: ({G * W}, vocab) with contiguous rows expected")
-    stride = logits.stride(0) if G * W > 1 else logits.shape[1]
-    st = _lib.load().qtip_beam_select(tokens.data_ptr(), parents.data_ptr(), scores.data_ptr(), logits.data_ptr(), _dtype_id(logits), stride,
-                                      prev_scores.data_ptr(), None if prev_tokens is None else prev_tokens.data_ptr(), G, W, logits.shape[1],
-                                      int(eos), _status_ptr(status), _stream())
-    _lib.check(st, "qtip_beam_select")
     global launch_count
-    launch_count += 1
+    launch_count += _lib.host().beam_select(tokens, parents, scores, logits, prev_scores, prev_tokens, eos, status)
 
 
 def beam_reorder(states, parents, lengths=None, status=None):
     """qtip_beam_reorder, in place: row b of each group becomes a copy of row parents[b] (parents (G, W) int32).  states: up to 8 of (tensor (G*W, outer,
     rows, values), tokens per row, modulus): of each of `outer` pieces the rows below length / tokens per row (length modulo the modulus where that
     is not 0) are copied; without lengths (G*W int32) all of them."""
-    _require_cuda(parents, lengths, status, *(t for t, _, _ in states))
-    _check_device(parents, lengths, status, *(t for t, _, _ in states))
-    G, W = parents.shape
-    _expect("parents", parents, torch.int32, (G, W))
-    if lengths is not None:
-        _expect("lengths", lengths, torch.int32, (G * W,))
-    arr = (_lib.BeamState * len(states))()
-    for c, (t, per_row, mod) in zip(arr, states):
-        if t.dim() != 4 or t.shape[0] != G * W or t.numel() == 0:
-            raise RuntimeError(f"a state is ({G * W}, outer, rows, values), not {tuple(t.shape)}")
-        if not t[0, 0].is_contiguous():
-            raise RuntimeError("the rows of a state have to be contiguous")
-        size = t.element_size()
-        c.base, c.seq_stride, c.outer_stride = t.data_ptr(), t.stride(0) * size, t.stride(1) * size
-        c.outer, c.rows, c.row_bytes, c.per_row, c.mod = t.shape[1], t.shape[2], t.shape[3] * size, per_row, mod
-    st = _lib.load().qtip_beam_reorder(arr, len(states), parents.data_ptr(), None if lengths is None else lengths.data_ptr(), G, W, _status_ptr(status),
-                                       _stream())
-    _lib.check(st, "qtip_beam_reorder")
     global launch_count
-    launch_count += 1
+    launch_count += _lib.host().beam_reorder(states, parents, lengths, status)

@@ -56,8 +56,7 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 
-// Exponentials are powers of two of x * kLog2e less a whole number, so that only the last sum is rounded.  The logarithm, divided by the same
-// constant, is off by its relative rounding (1.3e-8) times the entropy of the row.
+// exp(x - unit): the difference first (exact for what matters), so that logits of any size keep their distances.
 constexpr float kLog2e = 1.44269502162933349609375f;
 
 // A warp's batch in shared memory: vector j of lane l holds logits base + (j * 32 + l) * N + k; -inf behind the end of the slice.  A lane reads what
@@ -102,7 +101,7 @@ struct Batch {
         }
         return top;
     }
-    // Sum of 2^(x * kLog2e - unit), and the largest.
+    // Sum of exp(x - unit), and the largest.
     __device__ __forceinline__ float sum(float unit, float &top, int lane) const {
         float s[4] = {}, t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -112,7 +111,7 @@ struct Batch {
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 float e;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(x[k], kLog2e, -unit)));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[k] - unit) * kLog2e));
                 s[k & 3] += e;
                 t[k & 3] = fmaxf(t[k & 3], x[k]);
             }
@@ -165,15 +164,15 @@ __global__ void __launch_bounds__(kSelectThreads, 3) beam_select_kernel(const Se
             float top;
             if (__any_sync(kFullMask, unit == -INFINITY)) {
                 top = x.largest(lane);
-                if (unit == -INFINITY && fabsf(top) < INFINITY) unit = ceilf(top * kLog2e);
+                if (unit == -INFINITY && fabsf(top) < INFINITY) unit = top;
             }
             float more = x.sum(unit == -INFINITY ? 0.f : unit, top, lane);
             if (__any_sync(kFullMask, !(more <= 3.0e38f))) {           // an infinity or NaN, which do not count, or a change of the unit
                 x.only_finite(lane);
                 top = x.largest(lane);
                 const float old = unit;
-                if (top > -INFINITY) unit = fmaxf(unit, ceilf(top * kLog2e));
-                if (old > -INFINITY) sum *= exp2f(old - unit);
+                unit = fmaxf(unit, top);
+                if (old > -INFINITY) sum *= exp2f((old - unit) * kLog2e);
                 more = x.sum(unit == -INFINITY ? 0.f : unit, top, lane);
             }
             sum += more;
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(kSelectThreads, 3) beam_select_kernel(const Se
         float all = unit;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFullMask, all, o));
-        sum = unit > -INFINITY ? sum * exp2f(unit - all) : 0.f;
+        sum = unit > -INFINITY ? sum * exp2f((unit - all) * kLog2e) : 0.f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
         unit = all;
@@ -254,11 +253,11 @@ __global__ void __launch_bounds__(kSelectThreads, 3) beam_select_kernel(const Se
         double s = 0.0;
         for (int i = lane; i < per; i += 32) {
             const float2 v = S.sums[row * per + i];
-            if (v.y > 0.f) s += (double)v.y * (double)exp2f(v.x - mx);
+            if (v.y > 0.f) s += (double)v.y * (double)exp2f((v.x - mx) * kLog2e);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-        const double lse = (double)(float)(((double)mx + log2(s)) / (double)kLog2e);
+        const double lse = (double)(float)((double)mx + log(s));
         unsigned long long k[kSelectWarps / 32];
 #pragma unroll
         for (int e = 0; e < kSelectWarps / 32; e++) {

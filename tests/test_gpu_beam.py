@@ -1,0 +1,317 @@
+"""GPU: beam selection and reordering against a plain restatement, and QtipLlama's batch over the 8-bit cache and with beams."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as R
+from qtip_b200 import ops
+from qtip_b200.llama import LlamaShape, QtipLlama
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def select(logits, prev_scores, prev_tokens, eos, status=None):
+    G, W = prev_scores.shape
+    tokens, parents, scores = torch.full((G, W), -9, dtype=torch.int64, device=DEV), torch.full((G, W), -9, dtype=torch.int32, device=DEV), torch.zeros(G, W, device=DEV)
+    ops.beam_select(tokens, parents, scores, logits, prev_scores, prev_tokens, eos, status=status)
+    torch.cuda.synchronize()
+    return tokens.cpu(), parents.cpu(), scores.cpu()
+
+
+def check_select(logits, prev_scores, prev_tokens=None, eos=-1):
+    """Tokens and parents are equal; scores are sums in 64 bits of fp32 numbers, rounded once, the logarithm itself rounded to fp32 from a sum whose terms
+    have the exponential's error of 2^-22: one fp32 step of the logarithm (up to 2^-20 at 16) and half a step of the score."""
+    G, W = prev_scores.shape
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    dev_tokens = None if prev_tokens is None else prev_tokens.to(DEV)
+    tokens, parents, scores = select(logits.to(DEV), prev_scores.to(DEV), dev_tokens, eos, status)
+    none_at_all = False
+    for g in range(G):
+        t, p, sc, none = R.select(logits[g * W:(g + 1) * W].cpu(), prev_scores[g], prev_tokens[g] if prev_tokens is not None else None, eos)
+        none_at_all |= none
+        assert tokens[g].tolist() == t and parents[g].tolist() == p, g
+        for a, b in zip(scores[g].tolist(), sc):
+            assert a == b or abs(a - b) <= 2.0 ** -20 + 2.0 ** -24 * abs(b), (g, a, b)
+    assert int(status) == (2 if none_at_all else 0)
+
+
+@pytest.mark.parametrize("G, W, V", [(1, 1, 1), (1, 1, 50257), (2, 3, 3), (3, 2, 1000), (1, 4, 32000), (5, 5, 32001), (2, 8, 128256), (70, 3, 999), (1, 16, 40000), (40, 16, 129),
+                                     (300, 2, 2047), (9, 7, 8195)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_select_random(G, W, V, dtype):
+    g = torch.Generator().manual_seed(G * V + W)
+    logits = (2.5 * torch.randn(G * W, V, generator=g)).to(dtype)
+    scores = -10 * torch.rand(G, W, generator=g)
+    tokens = torch.randint(0, max(V, 2), (G, W), generator=g)
+    check_select(logits, scores, tokens, eos=1 if V > 2 else -1)
+
+
+def test_select_strides_and_in_place():
+    """Rows inside a wider buffer, not aligned; the same buffers for what was and what is."""
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(8, 1003, generator=g)
+    scores, tokens = -5 * torch.rand(2, 4, generator=g), torch.randint(3, 900, (2, 4), generator=g)
+    tokens[1, 2] = 2
+    check_select(wide[:, 3:1000], scores, tokens, eos=2)
+    d, s, t = wide.to(DEV)[:, 3:1000], scores.to(DEV), tokens.to(DEV)
+    p = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+    want = select(d, scores.to(DEV), tokens.to(DEV), 2)
+    ops.beam_select(t, p, s, d, s, t, 2)
+    assert torch.equal(t.cpu(), want[0]) and torch.equal(p.cpu(), want[1]) and torch.equal(s.cpu(), want[2])
+
+
+@pytest.mark.parametrize("W", [1, 4, 16])
+def test_select_equal_logits(W):
+    """Ties: the lower beam, then the lower token; rows that are one value, two values, rising, falling."""
+    V = 5000
+    rows = [torch.zeros(V), (torch.arange(V) % 2).float(), torch.arange(V).float() / 100, -torch.arange(V).float() / 100]
+    logits = torch.stack([rows[i % 4] for i in range(4 * W)])
+    check_select(logits, torch.zeros(4, W))
+    check_select(torch.cat([-logits.abs() * 0.0, logits * 0.0]), torch.zeros(8, W))            # -0 and 0
+
+
+def test_select_not_finite():
+    """Infinities, NaN, rows without a finite logit, beams without a score, groups without a continuation, far logits."""
+    W, V, nan, inf = 4, 3000, float("nan"), float("inf")
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(6 * W, V, generator=g)
+    x[0, ::3] = nan
+    x[1, 5:2000] = inf
+    x[2] = -inf
+    x[3, 7] = inf
+    x[4:8] = -inf                            # group 1: nothing
+    x[8] = -inf
+    x[8, 2999] = -300.0                      # one, far below, in the last place
+    x[9] = -inf
+    x[9, 0], x[9, 2000] = -1e30, 1e30
+    x[10, :2900] = -1e4
+    x[11] = nan
+    x[12:16] *= 1e4                          # group 3
+    scores = torch.zeros(6, W)
+    scores[4] = torch.tensor([0.0, -inf, nan, inf])
+    scores[5] = -inf
+    check_select(x, scores)
+
+
+def test_select_first_step_and_ended():
+    """One live beam fills the group; ended beams stay and take one row."""
+    g = torch.Generator().manual_seed(7)
+    scores = torch.full((3, 5), -math.inf)
+    scores[:, 0] = 0.0
+    check_select(torch.randn(15, 700, generator=g), scores)
+    tokens = torch.randint(3, 600, (3, 5), generator=g)
+    tokens[0], tokens[1, 2] = 2, 2
+    check_select(torch.randn(15, 700, generator=g), -torch.rand(3, 5, generator=g), tokens, eos=2)
+    check_select(torch.randn(3, 700, generator=g), torch.zeros(3, 1), torch.full((3, 1), 2), eos=2)
+
+
+def test_select_fewer_tokens_than_beams():
+    scores = torch.full((2, 6), -math.inf)
+    scores[:, 0] = -1.0
+    check_select(torch.randn(12, 4, generator=torch.Generator().manual_seed(8)), scores)
+
+
+def test_select_refusals():
+    G, W, V = 2, 4, 50
+    z = lambda dt: torch.zeros(G, W, dtype=dt, device=DEV)  # noqa: E731
+    ok = [z(torch.int64), z(torch.int32), z(torch.float32), torch.zeros(G * W, V, device=DEV), z(torch.float32), z(torch.int64), 2]
+    ops.beam_select(*ok)
+    for i, v, match in ((3, ok[3].double(), "unsupported dtype"), (3, ok[3][:7], "logits"), (3, torch.zeros(G * W, 2 * V, device=DEV)[:, ::2], "contiguous"), (0, z(torch.int32), "Long expected"),
+                        (1, z(torch.int64), "Int expected"), (4, z(torch.float32)[:1], "shape"), (5, None, "bad argument"), (3, ok[3].cpu(), "CUDA tensors only"),
+                        (3, ok[3][:1].expand(G * W, V), "shape")):
+        with pytest.raises(RuntimeError, match=match):
+            ops.beam_select(*(ok[:i] + [v] + ok[i + 1:]))
+    z17 = lambda dt: torch.zeros(1, 17, dtype=dt, device=DEV)  # noqa: E731
+    with pytest.raises(RuntimeError, match="shape"):
+        ops.beam_select(z17(torch.int64), z17(torch.int32), z17(torch.float32), torch.zeros(17, V, device=DEV), z17(torch.float32))
+
+
+# ------------------------------------------------------------------------------------------------------------- reordering
+def reordered(t, parents, lengths, per_row, mod):
+    out = t.clone()
+    G, W = parents.shape
+    for row in range(G * W):
+        p = row // W * W + int(parents[row // W, row % W])
+        n = t.shape[2]
+        if lengths is not None:
+            n = int(lengths[p]) % mod if mod else int(lengths[p])
+            n = min(-(-n // per_row), t.shape[2])
+        if p != row:
+            out[row, :, :n] = t[p, :, :n]
+    return out
+
+
+@pytest.mark.parametrize("W", [1, 2, 3, 8, 16])
+@pytest.mark.parametrize("kind", ["survivors", "any", "permutation", "one"])
+def test_reorder(W, kind):
+    """Any parents, rows that change places among them; pieces that are not a multiple of 16 bytes, strided and unaligned states; lengths that end inside
+    a column; rows behind them stay."""
+    G = 3
+    g = torch.Generator().manual_seed(W)
+    parents = torch.randint(0, W, (G, W), generator=g, dtype=torch.int32)
+    if kind == "survivors":
+        for b in range(G):
+            parents[b] = parents[b][parents[b].long()]
+            keep = parents[b].unique()
+            parents[b, keep.long()] = keep
+    if kind == "permutation":
+        parents = torch.stack([torch.randperm(W, generator=g) for _ in range(G)]).int()
+    if kind == "one":
+        parents[:] = W - 1
+    rnd = lambda *shape: torch.randint(0, 30000, shape, generator=g).to(torch.int16)  # noqa: E731
+    wide = rnd(G * W, 5, 70, 64)
+    states = [(rnd(G * W, 4, 33, 40), 1, 0), (rnd(G * W, 1, 9, 2), 16, 0), (wide[:, 1:3, 3:40], 2, 32), (rnd(G * W, 1, 2100, 128), 1, 0),
+              (rnd(G * W, 3, 7, 8).view(torch.int64).view(G * W, 3, 7, 2), 1, 5)]
+    for lengths in (None, torch.randint(0, 2200, (G, 1), generator=g, dtype=torch.int32).expand(G, W).reshape(-1).contiguous(),
+                    torch.randint(0, 40, (G * W,), generator=g, dtype=torch.int32)):
+        want = [reordered(t, parents, lengths, a, m) for t, a, m in states]
+        wide_dev = wide.to(DEV)
+        live = [(wide_dev[:, 1:3, 3:40] if i == 2 else t.to(DEV), a, m) for i, (t, a, m) in enumerate(states)]
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        ops.beam_reorder(live, parents.to(DEV), None if lengths is None else lengths.to(DEV), status=status)
+        torch.cuda.synchronize()
+        assert int(status) == 0
+        for (t, _, _), w in zip(live, want):
+            assert torch.equal(t.cpu(), w)
+        rest = wide_dev.cpu()
+        rest[:, 1:3, 3:40] = wide[:, 1:3, 3:40]
+        assert torch.equal(rest, wide)
+
+
+def test_reorder_parents_outside_and_refusals():
+    t = torch.arange(4 * 2 * 3 * 8, dtype=torch.int32, device=DEV).view(4, 2, 3, 8)
+    before, status = t.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    parents = torch.tensor([[7, -1, 0, 3]], dtype=torch.int32, device=DEV)
+    ops.beam_reorder([(t, 1, 0)], parents, status=status)
+    assert int(status) == 32 and torch.equal(t[[0, 1, 3]], before[[0, 1, 3]]) and torch.equal(t[2], before[0])
+    ok = [(t, 1, 0)]
+    for states, match in (([], "states"), (ok * 9, "states"), ([(t, 0, 0)], "out of range"), ([(t, 1, -1)], "out of range"), ([(t[:3], 1, 0)], "a state is"),
+                          ([(t.transpose(2, 3), 1, 0)], "contiguous"), ([(t[..., :4], 1, 0)], "contiguous"), ([(t.to(torch.int8)[..., :1].contiguous(), 1, 0)], "shape"),
+                          ([(t[:1].expand(4, 2, 3, 8), 1, 0)], "shape"), ([(t.cpu(), 1, 0)], "CUDA tensors only"), ([t], "tuple|state is")):
+        with pytest.raises(RuntimeError, match=match):
+            ops.beam_reorder(states, parents)
+    now = t.clone()
+    ops.beam_reorder(ok, parents.long()[:, :4].int().repeat(1, 2)[:, :4].t())        # four groups of one beam: nothing to do
+    assert torch.equal(t, now)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.beam_reorder(ok, torch.zeros(2, 2, dtype=torch.int32, device=DEV).t())
+
+
+# ------------------------------------------------------------------------------------------------------------ in the model
+SMALL = LlamaShape(n_layers=2, hidden=512, n_heads=4, n_kv_heads=2, head_dim=128, mlp=1376, vocab=700, K=2)
+
+
+def batch_logits(kv, B, steps, **kw):
+    model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=21)
+    model.enable_batch(B, kv=kv, **kw)
+    g, seen = torch.Generator().manual_seed(1), []
+    model.b_pos.copy_(torch.tensor([0] * B))
+    for _ in range(steps):
+        model.b_token.copy_(torch.randint(0, SMALL.vocab, (B,), generator=g))
+        model.step_batch()
+        seen.append(model.b_logits.clone())
+    model.check_status()
+    return torch.stack(seen)
+
+
+@pytest.mark.parametrize("kv, bound", [("int8", 0.03), ("e4m3", 0.12)])
+def test_batch_over_the_8_bit_cache(kv, bound):
+    """The same tokens through the batch over an fp16 cache and over the 8-bit one, up to 40 positions of blocks of 16.  A key or value is off by half of
+    1/127 of the block's largest (4 deviations: 0.016 of one, spread over half a step 0.009) for int8, by 2^-4 of itself at most (0.026 spread) for e4m3;
+    the logits may differ by about three times that."""
+    exact, got = batch_logits(None, 3, 40), batch_logits(kv, 3, 40, block=16)
+    first = (got[:15] - exact[:15]).norm() / exact[:15].norm()
+    rest = (got[15:] - exact[15:]).norm() / exact[15:].norm()
+    assert float(first) < 0.005          # nothing is in 8 bits yet: the angle's rounding alone
+    assert float(rest) < bound
+
+
+def plain_beams(model, W, prompt, steps, eos):
+    """Beam search by hand: every step's logits of every beam from its whole token list, one sequence at a time."""
+    beams, tokens = [(0.0, list(prompt))] + [(-math.inf, list(prompt))] * (W - 1), None
+    for _ in range(steps):
+        rows = []
+        for _, toks in beams:
+            model.reset()
+            model.feed(torch.tensor(toks))
+            rows.append(model.logits[0].clone())
+        x = torch.stack(rows)
+        last = torch.tensor([t[-1] for _, t in beams])
+        toks, parents, scores, _ = R.select(x.cpu(), torch.tensor([b[0] for b in beams]), last, eos)
+        beams = [(s, beams[p][1] + [t]) for t, p, s in zip(toks, parents, scores)]
+    return beams
+
+
+@pytest.mark.parametrize("kv", [None, "int8"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_beams_in_the_model(kv, captured):
+    """Two groups of three beams over 40 steps: the scores are those of the tokens, evaluated again by a batch without beams; the graph gives the eager
+    run's tokens; sequences that share blocks read what their parents wrote."""
+    W, steps, prompts = 3, 40, torch.tensor([[5, 6, 7], [300, 200, 100]])
+    model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=22)
+    model.enable_batch(6, kv=kv, block=16)
+    model.enable_beams(W, eos=-1)
+    if captured:
+        model.capture_batch()
+    model.feed_beams(prompts)
+    model.generate_batch(steps)
+    model.check_status()
+    tokens, scores = model.b_out_tokens[:, :3 + steps + 1].clone(), model.b_scores.clone()
+    assert model.b_pos.tolist() == [3 + steps] * 6
+    for row in range(6):
+        assert tokens[row, :3].tolist() == prompts[row // W].tolist()
+    again = QtipLlama(SMALL, max_positions=64, device=DEV, seed=22)
+    again.enable_batch(6, kv=kv, block=16)
+    total = torch.zeros(6, dtype=torch.float64, device=DEV)
+    for i in range(3 + steps):
+        again.b_token.copy_(tokens[:, i])
+        again._forward_batch()
+        again.b_pos.add_(1)
+        if i >= 2:
+            total += torch.log_softmax(again.b_logits.double(), 1).gather(1, tokens[:, i + 1:i + 2]).view(-1)
+    # 41 sums of scores, each with a logarithm and a score rounded to fp32 (2^-21 and 2^-17 at 300)
+    assert float((total.view(2, W) - scores.double()).abs().max()) < 41 * (2.0 ** -20 + 2.0 ** -17)
+    assert len({tuple(t) for t in tokens.tolist()}) == 6
+
+
+def test_beams_follow_a_search_by_hand():
+    """Two beams, six steps, one sequence at a time through the batch-1 step over the fp16 cache.  (Its kernels add in another order: a seed whose
+    choices are not close, scores within 2 %.)"""
+    shape = SMALL
+    model = QtipLlama(shape, max_positions=32, device=DEV, seed=23)
+    want = plain_beams(model, 2, [11, 12], 4, -1)
+    model.enable_batch(2, kv="int8", block=16)
+    model.enable_beams(2)
+    model.feed_beams(torch.tensor([[11, 12]]))
+    model.generate_batch(3)
+    got = sorted(zip(model.b_scores.view(-1).tolist(), model.b_out_tokens[:, :6].tolist()))
+    for (a, t), (b, u) in zip(got, sorted((s, t) for s, t in want)):
+        assert t == u and abs(a - b) < 0.02 * abs(b)
+
+
+def test_beams_end():
+    """Every token may end a beam: with eos as the likeliest token all beams end, keep their score and repeat it."""
+    model = QtipLlama(SMALL, max_positions=32, device=DEV, seed=24)
+    model.enable_batch(4, kv="e4m3", block=16)
+    model.enable_beams(4)
+    model.feed_beams(torch.tensor([[1, 2]]))
+    eos = int(model.b_token[0])
+    model.beam_eos = eos
+    ended = (model.b_token == eos).nonzero().view(-1).tolist()
+    before = [float(model.b_scores.view(-1)[r]) for r in ended]
+    model.generate_batch(5)
+    model.check_status()
+    scores, tokens = model.b_scores.view(-1).tolist(), model.b_out_tokens[:, :8].tolist()
+    assert any(s == before[0] and t[2:] == [eos] * 6 for s, t in zip(scores, tokens))
+
+
+def test_pool_smaller_than_the_sequences():
+    """A pool without room: the status says so, and the batch runs on with what it has."""
+    model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=25)
+    model.enable_batch(2, kv="int8", block=16, n_blocks=3)
+    for _ in range(34):
+        model.step_batch()
+    with pytest.raises(RuntimeError, match="8 = no free block"):
+        model.check_status()

@@ -4,8 +4,8 @@
 // Bound by the bytes of the cache: 2 per token, key/value head and dim, read once for all query heads that share them.
 // A pair is a sequence and a key/value head (of at most 16 query heads; more are further pairs).  Its tokens are cut into tiles of 32, and the
 // tiles of all pairs, in order, are dealt to the CTAs in equal contiguous ranges, computed by every CTA from the lengths: a long sequence is
-// spread over the chip, and a CTA goes through several short ones.  A cut that would leave less than kSnap + 1 tiles on one side is moved
-// to the pair's border.  A pair inside one range is finished there; the parts of others go to the workspace, and a second kernel joins
+// spread over the chip, and a CTA goes through several short ones.  The start of a pair counts as kStart tiles (its queries, and the join of the
+// four warps' sums).  A cut that would leave less than kSnap + 1 tiles on one side is moved to the pair's border.  A pair inside one range is finished there; the parts of others go to the workspace, and a second kernel joins
 // them in the order of the tokens.
 // A warp takes every fourth tile of a range.  One of its lanes keeps kStages copies of tiles in flight (a tile of a block of 32 tokens or
 // more is one piece of memory: K and V of 32 tokens); the lanes read the bytes in the order of the operands of the matrix instruction
@@ -18,13 +18,9 @@
 namespace qtip {
 namespace {
 
-constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kTile = 32, kSnap = 4, kRowsMax = 16;
-#ifndef KW
-#define KW 3
-#define KC 64
-#define KF 60
-#endif
-constexpr int kWaves = KW, kChunk = KC, kFirst = KF;
+constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kTile = 32, kSnap = 4, kStart = 4, kRowsMax = 16;
+// Waves of CTAs for much work, the share of the first in %, and how much is much: bytes of a CTA's tiles, if there were one wave.
+constexpr int kWaves = 3, kFirst = 60, kMuch = 160 * 8192;
 constexpr float kLift = 15.f;        // weights are 2^15 times exp(score - maximum): fp16 then reaches down to 2^-39 of the largest
 constexpr unsigned kPolls = 1u << 20;
 constexpr int kStatusWait = 64;
@@ -102,9 +98,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
 
 constexpr int kTailTile = 16;      // tokens of a tile of the tail: as many bytes as 32 in 8 bits
 
-// A sequence's tokens in blocks, all of them, and tiles of either.
+// A sequence's tokens in blocks, all of them, and tiles of either; what one of its pairs counts.
 struct Sequence {
     int full, len, coded, tiles;
+    __device__ __forceinline__ int cost() const { return tiles ? tiles + kStart : 0; }
 };
 __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int len) {
     Sequence q;
@@ -119,7 +116,7 @@ __device__ __forceinline__ int length_of(const AttnArgs &a, int s) {
     return len < 0 || len >> a.shift > a.max_blocks ? 0 : len;
 }
 
-// A walk over the parts of pairs in a range of tiles: sequence, pair of it, the part's tiles t0 .. t1, and the range's tiles from t0 on.
+// A walk over the parts of pairs in a range: sequence, pair of it, the part's tiles t0 .. t1, and what the range counts from t0 on.
 struct Walk {
     int s, i, t0, t1, left;
     Sequence q;
@@ -156,9 +153,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
     const int per = (a.n_seqs + 31) >> 5, s_lo = min(lane * per, a.n_seqs), s_hi = min(s_lo + per, a.n_seqs);
     int mine = 0, seqs = 0;
     for (int s = s_lo; s < s_hi; s++) {
-        const int tiles = sequence(a, length_of(a, s)).tiles;
-        mine += tiles;
-        seqs += tiles > 0;
+        const int cost = sequence(a, length_of(a, s)).cost();
+        mine += cost;
+        seqs += cost > 0;
     }
     int upto = mine;
 #pragma unroll
@@ -172,7 +169,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
     // CTAs per further wave equal ranges of the rest, as the first ones end: some SMs get at the memory faster than others.
     const int least = max(total / kAttnWarps, seqs * pairs), room = gridDim.x / kWaves;
     int ctas = max(min(min(total, least), room), 1), share2 = 0, rest2 = 0, early = ctas, early_tiles = total;
-    if (kWaves > 1 && total >= room * kChunk) {
+    if (kWaves > 1 && total >= room * (kMuch / kTileBytes)) {
         ctas = gridDim.x;
         early = room;
         early_tiles = total / 100 * kFirst;
@@ -180,10 +177,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
         rest2 = total - early_tiles - share2 * (ctas - early);
     }
     const int share = early_tiles / early, rest = early_tiles - share * early;
-    auto border = [&](int cta) {                       // first tile of a CTA's range, before it is moved to a pair's border
+    auto border = [&](int cta) {                       // where a CTA's range begins, before it is moved to a pair's border
         return cta <= early ? cta * share + min(cta, rest) : early_tiles + (cta - early) * share2 + min(cta - early, rest2);
     };
-    auto owner = [&](int tile) {                       // the last CTA whose border is not behind the tile
+    auto owner = [&](int tile) {                       // the last CTA whose border is not behind this
         const int base = tile < early_tiles ? 0 : early, n = tile < early_tiles ? share : share2, r = tile < early_tiles ? rest : rest2;
         if (tile >= early_tiles) tile -= early_tiles;
         return base + (tile < r * (n + 1) ? tile / (n + 1) : (tile - r) / n);
@@ -205,17 +202,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
         if (here) {
             int before = (upto - mine) * pairs;
             for (int s = s_lo; s < s_hi; s++) {
-                const int len = length_of(a, s), tiles = sequence(a, len).tiles;
-                if (at < before + tiles * pairs) {
+                const int len = length_of(a, s), cost = sequence(a, len).cost();
+                if (at < before + cost * pairs) {
                     ps = s;
                     plen = len;
-                    pi = (at - before) / tiles;
-                    px = at - before - pi * tiles;
-                    if (px <= kSnap) { at -= px; px = 0; }
-                    else if (tiles - px <= kSnap) { at += tiles - px; px = 0; pi++; }
+                    pi = (at - before) / cost;
+                    px = at - before - pi * cost;
+                    if (px <= kStart + kSnap) { at -= px; px = 0; }
+                    else if (cost - px <= kSnap) { at += cost - px; px = 0; pi++; }
+                    else px -= kStart;
                     break;
                 }
-                before += tiles * pairs;
+                before += cost * pairs;
             }
         }
         const unsigned who = __ballot_sync(kFullMask, here);      // none for the end of all tiles
@@ -240,7 +238,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
     };
     if (w.i >= pairs) next_pair(w);
     w.left = length;
-    w.t1 = min(w.q.tiles, w.t0 + w.left);
+    auto bound = [&](Walk &y) { y.t1 = min(y.q.tiles, y.t0 ? y.t0 + y.left : y.left - kStart); };
+    auto count = [](const Walk &y) { return y.t1 - y.t0 + (y.t0 ? 0 : kStart); };          // of the part
+    bound(w);
 
     // ---- copies of this warp's tiles, kStages ahead
     Walk ahead = w;
@@ -248,10 +248,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
     bool more = true;
     auto settle = [&]() {                // to this warp's next tile, and its blocks' numbers
         while (more && ahead_t >= ahead.t1) {
-            ahead.left -= ahead.t1 - ahead.t0;
+            ahead.left -= count(ahead);
             if (ahead.left <= 0) { more = false; break; }
             next_pair(ahead);
-            ahead.t1 = min(ahead.q.tiles, ahead.left);
+            bound(ahead);
             ahead_t = warp;
             ahead_h = ahead.i / a.groups;
         }
@@ -608,10 +608,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
             // the CTAs from this one to the one that ends the pair
             int parts = 0;
             if (!whole) {
-                const int begins = from + (length - w.left), end = begins + w.q.tiles;
+                const int begins = from + (length - w.left), end = begins + w.q.cost();
                 int last = owner(end - 1);
                 for (; last > (int)blockIdx.x; last--) {
-                    const int x = border(last) - begins;           // its range begins inside this pair
+                    const int x = border(last) - begins - kStart;      // its range begins inside this pair
                     if (x > kSnap && w.q.tiles - x > kSnap) break;
                 }
                 parts = last - (int)blockIdx.x + 1;
@@ -619,10 +619,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
             a.meta[s * pairs + w.i] = make_int2(slot, parts);
         }
         first = false;
-        w.left -= w.t1 - w.t0;
+        w.left -= count(w);
         if (w.left <= 0) break;
         next_pair(w);
-        w.t1 = min(w.q.tiles, w.left);
+        bound(w);
     }
     if (!waited) {                       // a copy did not arrive in time: report, and leave only when none is in flight
         if (a.status && lane == 0) atomicOr(a.status, (unsigned)kStatusWait);
@@ -731,7 +731,7 @@ extern "C" int qtip_attn_decode_paged(void *out, long out_stride, const void *q,
     if (((long)max_blocks + 1) * block > 0x7FFFFFFFl) return QTIP_ERR_BAD_SHAPE;
     const Workspace ws = workspace_of(n_seqs, n_heads, n_kv_heads, head_dim);
     const int most = (int)(((long)max_blocks * block + kTile - 1) / kTile) + block / kTailTile;                // tiles of a pair
-    if ((long)most * n_seqs * n_kv_heads * ws.groups > 0x3FFFFFFFl) return QTIP_ERR_TOO_LARGE;          // tiles are counted in 32 bits
+    if ((long)(most + kStart) * n_seqs * n_kv_heads * ws.groups > 0x3FFFFFFFl) return QTIP_ERR_TOO_LARGE;          // tiles are counted in 32 bits
     if (!workspace || workspace_bytes < ws.bytes) return QTIP_ERR_WORKSPACE;
     const void *ptrs[] = {out, q, data, scales, tail_k, tail_v, workspace};
     for (const void *p : ptrs)

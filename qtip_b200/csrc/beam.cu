@@ -9,11 +9,11 @@ constexpr int kMaxBeams = 16, kMaxStates = 8;
 
 // ---- selection -------------------------------------------------------------------------------------------------------------------
 // A group's beams w < W with scores c_w and logits x_w: the W largest of c_w + (x_wv - lse_w), lse_w = log sum_v exp x_wv.
-// One cluster per group; its warps share the rows.  A warp reads its slice once, in batches of 32 logits per lane that are copied to shared memory
+// One cluster per group; its warps share the rows.  A warp reads its slice once, in batches of 24 logits per lane that are copied to shared memory
 // one batch ahead: the sum of exponentials with a running maximum in each lane, and the W largest logits, sorted in its lanes.  A batch without
 // a logit above the last of these costs one comparison; in the first batch the W-th largest of the lanes' largest is the bound.  CTA 0
 // merges the lists of a row, one warp per row, adds scores in 64 bits and takes the W largest of the W * W continuations that are left.
-constexpr int kSelectThreads = 256, kSelectCluster = 16, kSelectWarps = kSelectThreads / 32 * kSelectCluster, kSelectHeld = 32, kSelectStages = 2;
+constexpr int kSelectThreads = 256, kSelectCluster = 16, kSelectWarps = kSelectThreads / 32 * kSelectCluster, kSelectHeld = 24, kSelectStages = 2;
 
 struct SelectArgs {
     long long *tokens;
@@ -129,7 +129,7 @@ struct Batch {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kSelectThreads, 3) beam_select_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kSelectThreads, 4) beam_select_kernel(const SelectArgs a) {
     extern __shared__ __align__(16) uint8_t select_smem[];
     SelectSmem &S = *reinterpret_cast<SelectSmem *>(select_smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.width, g = blockIdx.y;
@@ -494,8 +494,8 @@ constexpr size_t select_smem_bytes() {
     return ring > sizeof(SelectSmem) ? ring : sizeof(SelectSmem);
 }
 
-// CTAs of a group: 1 to 16 (8 where the GPU has no room for clusters of 16), so that the rounds of clusters that the chip holds at once, each as long
-// as a warp's part of a row, take the least time.
+// CTAs of a group: as many as the chip holds at once for all groups; more would be a second round.  64 groups of 8 beams over 128256 tokens take
+// 74 us with 4 and 60 with 8; one group 28 us with 8 and 21 with 16 (where the GPU has room for clusters of 16).
 template <typename T>
 int launch_select(const SelectArgs &a, int groups, cudaStream_t stream) {
     static int cached[64][5] = {};       // clusters of 1, 2, 4, 8, 16 CTAs at once, plus one
@@ -528,7 +528,8 @@ int launch_select(const SelectArgs &a, int groups, cudaStream_t stream) {
             }
             if (dev < 64) cached[dev][k] = n + 1;
         }
-        const double time = n ? (double)((groups + n - 1) / n) / per : 1e30;
+        if (c == 16 && n < groups) continue;
+        const double time = n ? (double)((groups + n - 1) / n) / per : 1e30;               // rounds, each as long as a warp's part of a row
         if (!cluster || time < best) { cluster = c; best = time; }
     }
     cfg.gridDim = dim3(cluster, groups);

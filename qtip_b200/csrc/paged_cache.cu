@@ -9,10 +9,13 @@ namespace qtip {
 namespace {
 
 // ---- block tables and runs -------------------------------------------------------------------------------------------------------
-// One CTA.  A block is free when no sequence's table names it among its complete blocks (a bitmap in shared memory): there is no free
+// A block is free when no sequence's table names it among its complete blocks (a bitmap in shared memory): there is no free
 // list to keep, a sequence whose length is set to zero has released its blocks, and tables that name the same block (beams of one
 // search, a common prompt) share it.  The new blocks are the lowest free ones, in the order of the sequences.
-constexpr int kPlanThreads = 1024, kPlanLoads = 8, kPlanMaxBlocks = 1600000, kPlanMaxTokens = 1 << 20;
+// One CTA; for many table entries a cluster of eight, each of which marks every eighth share of 32 sequences in a bitmap of its own, which the first
+// then takes over (marking is bound by the shared-memory atomics of an SM: 512 sequences with 130000 blocks 31 us with one CTA, 18 with
+// eight; eight sequences of at most 128 blocks 5.4 with one).
+constexpr int kPlanThreads = 1024, kPlanLoads = 8, kPlanCluster = 8, kPlanEntries = 32768, kPlanMaxBlocks = 1600000, kPlanMaxTokens = 1 << 20;
 
 struct PlanArgs {
     int *tables;
@@ -55,12 +58,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = a.block;
     const int words = (a.n_blocks + 31) >> 5, per = (words + kPlanThreads - 1) / kPlanThreads;
     unsigned bad = 0;
+    const int ctas = gridDim.x, rank = blockIdx.x;           // one cluster
     for (int w = tid; w < words; w += kPlanThreads) {
         const int left = a.n_blocks - w * 32;
         held[w] = left >= 32 ? 0u : ~0u << left;             // places behind the pool's last block are never free
     }
     __syncthreads();
-    for (int s = warp; s < a.n_seqs; s += kPlanThreads / 32) {
+    for (int s = warp * ctas + rank; s < a.n_seqs; s += ctas * (kPlanThreads / 32)) {
         const int live = min(max(a.lengths[s], 0) / b, a.max_blocks);
         const int *row = a.tables + (size_t)s * a.max_blocks;
         for (int j0 = lane; j0 < live; j0 += 32 * kPlanLoads) {      // the loads of a step are in flight together
@@ -73,6 +77,29 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
                 if ((unsigned)id[u] < (unsigned)a.n_blocks) atomicOr(&held[id[u] >> 5], 1u << (id[u] & 31));
                 else bad |= 16u;
             }
+        }
+    }
+    if (ctas > 1) {
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        if (rank == 0)
+            for (int w = tid; w < words; w += kPlanThreads) {
+                const uint32_t at = (uint32_t)__cvta_generic_to_shared(held + w);
+                uint32_t v[kPlanCluster];
+#pragma unroll
+                for (int r = 1; r < kPlanCluster; r++) {
+                    uint32_t from;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(r));
+                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[r]) : "r"(from) : "memory");
+                }
+                uint32_t all = held[w];
+#pragma unroll
+                for (int r = 1; r < kPlanCluster; r++) all |= v[r];
+                held[w] = all;
+            }
+        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // the bitmaps are read
+        if (rank != 0) {
+            if (bad && a.status) atomicOr(a.status, bad);
+            return;
         }
     }
     __syncthreads();
@@ -390,7 +417,22 @@ extern "C" int qtip_kv_plan(int *tables, const int *lengths, const int *new_toke
     const PlanArgs a = {tables, lengths, new_tokens, lengths_out, runs, n_runs, n_seqs, max_blocks, n_blocks, block, n_tokens, status};
     const size_t smem = (size_t)((n_blocks + 31) / 32) * 4;
     if (smem > 16384) QTIP_CUDA_TRY(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanMaxBlocks + 31) / 32 * 4));
-    return launch_dependent(kv_plan_kernel, dim3(1), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), a);
+    const int ctas = (long)n_seqs * max_blocks < kPlanEntries ? 1 : kPlanCluster;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctas > 1 ? 2 : 1;
+    QTIP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_plan_kernel, a));
+    return check_launch();
 }
 
 extern "C" int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const void *q, long q_stride, const void *k, long k_stride, const void *v,

@@ -68,7 +68,7 @@ def check_plan(tables, lengths, new, n_blocks, block, n_tokens):
     assert bool((runs[n:] == 77).all())
 
 
-@pytest.mark.parametrize("seqs, block, n_blocks, hi", [(1, 128, 1, 100), (7, 16, 300, 300), (513, 32, 2500, 120), (2100, 16, 40000, 60), (130, 16, 70001, 3000)])
+@pytest.mark.parametrize("seqs, block, n_blocks, hi", [(1, 128, 1, 100), (7, 16, 300, 300), (513, 32, 2500, 120), (2100, 16, 40000, 60), (130, 16, 70001, 3000), (300, 16, 90000, 3000)])
 def test_plan_random(seqs, block, n_blocks, hi):
     """More sequences than threads, pools that are not a multiple of 32, tables that share blocks and name none, too few blocks at the end."""
     g = torch.Generator().manual_seed(seqs)

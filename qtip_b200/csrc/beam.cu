@@ -550,6 +550,9 @@ extern "C" int qtip_beam_select(long long *tokens, int *parents, float *scores, 
     if (!tokens || !parents || !scores || !logits || !prev_scores || (logits_dtype != QTIP_F16 && logits_dtype != QTIP_F32) || (eos >= 0 && !prev_tokens))
         return QTIP_ERR_BAD_ARG;
     if (groups < 1 || groups > 65535 || width < 1 || width > kMaxBeams || vocab < 1 || vocab > (1 << 30) || logits_stride < vocab) return QTIP_ERR_BAD_SHAPE;
+    if (!aligned(tokens, 8) || (prev_tokens && !aligned(prev_tokens, 8)) || !aligned(parents, 4) || !aligned(scores, 4) || !aligned(prev_scores, 4) ||
+        !aligned(status, 4) || !aligned(logits, logits_dtype == QTIP_F32 ? 4 : 2))
+        return QTIP_ERR_ALIGNMENT;
     const SelectArgs a = {tokens, parents, scores, logits, logits_stride, prev_scores, prev_tokens, width, vocab, eos, status};
     return logits_dtype == QTIP_F32 ? launch_select<float>(a, groups, static_cast<cudaStream_t>(stream))
                                     : launch_select<__half>(a, groups, static_cast<cudaStream_t>(stream));
@@ -559,6 +562,7 @@ extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, co
                                  unsigned *status, void *stream) {
     if (!states || !parents || n_states < 1 || n_states > kMaxStates) return QTIP_ERR_BAD_ARG;
     if (groups < 1 || groups > 65535 || width < 1 || width > kMaxBeams) return QTIP_ERR_BAD_SHAPE;
+    if (!aligned(parents, 4) || (lengths && !aligned(lengths, 4)) || !aligned(status, 4)) return QTIP_ERR_ALIGNMENT;
     ReorderArgs a = {};
     a.parents = parents;
     a.lengths = lengths;
@@ -569,6 +573,8 @@ extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, co
     for (int k = 0; k < n_states; k++) {
         const qtip_beam_state &s = states[k];
         if (!s.base) return QTIP_ERR_BAD_ARG;
+        for (int j = 0; j < k; j++)
+            if (states[j].base == s.base) return QTIP_ERR_BAD_ARG;              // it would be reordered twice
         if (s.outer < 1 || s.rows < 1 || s.row_bytes < 4 || s.per_row < 1 || s.mod < 0 || (s.row_bytes & 3) || (s.seq_stride & 3) || (s.outer_stride & 3) ||
             (long)s.rows * s.row_bytes > s.seq_stride || (s.outer > 1 && ((long)s.rows * s.row_bytes > s.outer_stride || (s.outer - 1) * s.outer_stride + (long)s.rows * s.row_bytes > s.seq_stride)))
             return QTIP_ERR_BAD_SHAPE;

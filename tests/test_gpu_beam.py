@@ -187,7 +187,7 @@ def test_reorder_parents_outside_and_refusals():
     ops.beam_reorder([(t, 1, 0)], parents, status=status)
     assert int(status) == 32 and torch.equal(t[[0, 1, 3]], before[[0, 1, 3]]) and torch.equal(t[2], before[0])
     ok = [(t, 1, 0)]
-    for states, match in (([], "states"), (ok * 9, "states"), ([(t, 0, 0)], "out of range"), ([(t, 1, -1)], "out of range"), ([(t[:3], 1, 0)], "a state is"),
+    for states, match in (([], "states"), (ok * 9, "states"), (ok * 2, "bad argument"), ([(t, 0, 0)], "out of range"), ([(t, 1, -1)], "out of range"), ([(t[:3], 1, 0)], "a state is"),
                           ([(t.transpose(2, 3), 1, 0)], "contiguous"), ([(t[..., :4], 1, 0)], "contiguous"), ([(t.to(torch.int8)[..., :1].contiguous(), 1, 0)], "shape"),
                           ([(t[:1].expand(4, 2, 3, 8), 1, 0)], "shape"), ([(t.cpu(), 1, 0)], "CUDA tensors only"), ([t], "tuple|state is")):
         with pytest.raises(RuntimeError, match=match):

@@ -22,7 +22,7 @@ def test_plan_arguments():
     for i, v in ((6, 0), (6, 65536), (7, 0), (8, 0), (8, 1600001), (9, 8), (9, 48), (9, 256), (10, -1), (10, (1 << 20) + 1), (7, 1 << 27)):
         assert st(i, v) == _lib.ERR_BAD_SHAPE, (i, v)
     assert st(11, 3) == _lib.ERR_WORKSPACE
-    assert st(4, P + 68) == _lib.ERR_ALIGNMENT
+    assert st(4, P + 68) == _lib.ERR_ALIGNMENT and st(0, P + 2) == _lib.ERR_ALIGNMENT and st(12, P + 1) == _lib.ERR_ALIGNMENT
 
 
 def test_append_arguments():
@@ -36,7 +36,7 @@ def test_append_arguments():
         assert st(i, None) == _lib.ERR_BAD_ARG
     for i, v in ((16, -1), (18, -1), (19, 0), (20, 0), (21, 0), (22, 96), (22, 256), (23, 0), (24, 24), (24, 8), (25, 2), (25, -1)):
         assert st(i, v) == _lib.ERR_BAD_SHAPE, (i, v)
-    for i, v in ((0, P + 8), (2, P + 2), (8, P + 8), (14, P + 4), (1, 68), (3, 65), (11, 2052)):
+    for i, v in ((0, P + 8), (2, P + 2), (8, P + 8), (14, P + 4), (1, 68), (3, 65), (11, 2052), (17, P + 4), (15, P + 2)):
         assert st(i, v) == _lib.ERR_ALIGNMENT, (i, v)
     assert st(18, 0) == _lib.OK and st(16, 0) == _lib.OK          # nothing to do
 
@@ -56,7 +56,7 @@ def test_attention_arguments():
     for i, v in ((12, 0), (12, 65536), (13, 7), (14, 0), (15, 32), (16, 0), (16, 1 << 27), (17, 0), (18, 20), (19, 2)):
         assert st(i, v) == _lib.ERR_BAD_SHAPE, (i, v)
     assert st(20, None) == _lib.ERR_WORKSPACE and st(21, need - 1) == _lib.ERR_WORKSPACE
-    for i, v in ((0, P + 8), (2, P + 4), (6, P + 8), (20, P + 4), (1, 516), (3, 513), (9, 2050)):
+    for i, v in ((0, P + 8), (2, P + 4), (6, P + 8), (20, P + 4), (1, 516), (3, 513), (9, 2050), (10, P + 2), (11, P + 1)):
         assert st(i, v) == _lib.ERR_ALIGNMENT, (i, v)
     big = lib.qtip_attn_paged_workspace_bytes(65535, 8, 2, 64)
     assert f(*(ok[:12] + [65535, 8, 2, 64, 1 << 20, 8, 16, 0, P, big, None, None])) == _lib.ERR_TOO_LARGE
@@ -75,6 +75,9 @@ def test_beam_arguments():
     for i, v in ((8, 0), (8, 65536), (9, 0), (9, 17), (10, 0), (5, 99), (10, (1 << 30) + 1)):
         assert st(i, v) == _lib.ERR_BAD_SHAPE, (i, v)
 
+    for i, v in ((0, P + 4), (1, P + 2), (2, P + 1), (3, P + 2), (6, P + 2), (7, P + 4), (12, P + 2)):
+        assert st(i, v) == _lib.ERR_ALIGNMENT, (i, v)
+
     def reorder(n=1, parents=P, groups=1, width=2, **kw):
         state = dict(base=P, seq_stride=64, outer_stride=64, outer=1, rows=2, row_bytes=32, per_row=1, mod=0, **{})
         state.update(kw)
@@ -84,7 +87,8 @@ def test_beam_arguments():
     for kw in (dict(groups=0), dict(width=17), dict(outer=0), dict(rows=0), dict(row_bytes=2), dict(row_bytes=30), dict(per_row=0), dict(mod=-1), dict(seq_stride=60),
                dict(seq_stride=66), dict(outer=2), dict(outer=2, seq_stride=128, outer_stride=32), dict(outer=2, seq_stride=128, outer_stride=66)):
         assert reorder(**kw) == _lib.ERR_BAD_SHAPE, kw
-    assert reorder(base=P + 2) == _lib.ERR_ALIGNMENT
+    assert reorder(base=P + 2) == _lib.ERR_ALIGNMENT and reorder(parents=P + 2) == _lib.ERR_ALIGNMENT
+    assert reorder(n=2) == _lib.ERR_BAD_ARG                       # the same state twice
     assert reorder(rows=1 << 28, seq_stride=1 << 34) == _lib.ERR_TOO_LARGE
     assert reorder(width=1) == _lib.OK                            # a beam alone has nowhere to go
 

@@ -57,7 +57,7 @@ __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 
 // exp(x - unit): the difference first (exact for what matters), so that logits of any size keep their distances.
-constexpr float kLog2e = 1.44269502162933349609375f;
+constexpr float kLog2e = 1.44269502162933349609375f, kSumTop = 4294967296.f;
 
 // A warp's batch in shared memory: vector j of lane l holds logits base + (j * 32 + l) * N + k; -inf behind the end of the slice.  A lane reads what
 // it copied itself.
@@ -160,14 +160,15 @@ __global__ void __launch_bounds__(kSelectThreads, 4) beam_select_kernel(const Se
             } else {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
-            // a lane's unit comes from its first finite logit's batch; a later one is above it by no more than fp32 can hold, or changes it
+            // A lane's unit is the largest logit of its first batch, until a batch's sum in that unit is above kSumTop (a logit some 20 above it), which
+            // raises it.  So a lane adds at most 2^21 batches of at most 2^32, 32 lanes 2^58: no sum leaves fp32.
             float top;
             if (__any_sync(kFullMask, unit == -INFINITY)) {
                 top = x.largest(lane);
                 if (unit == -INFINITY && fabsf(top) < INFINITY) unit = top;
             }
             float more = x.sum(unit == -INFINITY ? 0.f : unit, top, lane);
-            if (__any_sync(kFullMask, !(more <= 3.0e38f))) {           // an infinity or NaN, which do not count, or a change of the unit
+            if (__any_sync(kFullMask, !(more <= kSumTop))) {           // a change of the unit, or an infinity or NaN, which do not count
                 x.only_finite(lane);
                 top = x.largest(lane);
                 const float old = unit;

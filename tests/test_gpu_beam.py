@@ -95,6 +95,25 @@ def test_select_not_finite():
     check_select(x, scores)
 
 
+# Distances of a row's larger logits from those that a warp meets first: below, at and above what 32 bits can hold of an exponential (88.7).
+DISTANCES = [0, 5, 14, 20, 22, 23, 30, 40, 44, 45, 60, 70, 75, 78, 80, 81, 82, 82.5, 83, 83.5, 84, 84.5, 85, 85.3, 86, 87, 87.5, 88, 88.5, 89, 95, 120]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("low", ["first", "rising", "two values"])
+def test_select_distances(dtype, low):
+    """Logits that begin far below the rest of a slice, or rise through it in several batches: sums of exponentials neither overflow nor lose what counts.
+    A warp's slice is 4000 logits (or 2, 4, 8 times as many); one live beam in each group, so that a lost row shows as missing continuations."""
+    W, V, G = 16, 32000, len(DISTANCES)
+    at = torch.arange(V) % 4000
+    share = {"first": (at < 768).float(), "rising": 1 - at / 4000, "two values": (at < 768).float()}[low]
+    noise = torch.zeros(G * W, V) if low == "two values" else 0.5 * torch.randn(G * W, V, generator=torch.Generator().manual_seed(11))
+    logits = (noise - torch.tensor(DISTANCES).repeat_interleave(W).view(-1, 1) * share).to(dtype)
+    scores = torch.full((G, W), -math.inf)
+    scores[torch.arange(G), torch.arange(G) % W] = -1.0
+    check_select(logits, scores)
+
+
 def test_select_first_step_and_ended():
     """One live beam fills the group; ended beams stay and take one row."""
     g = torch.Generator().manual_seed(7)

@@ -21,7 +21,7 @@ namespace {
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kTile = 32, kSnap = 4, kStart = 4, kRowsMax = 16;
 // Waves of CTAs for much work, the share of the first in %, and how much is much: bytes of a CTA's tiles, if there were one wave.
 constexpr int kWaves = 3, kFirst = 60, kMuch = 160 * 8192;
-constexpr float kLift = 15.f;        // weights are 2^15 times exp(score - maximum): fp16 then reaches down to 2^-39 of the largest
+constexpr float kLift = 32768.f;     // weights are multiplied by 2^15 before they are rounded: fp16 then reaches down to 2^-39 of the largest
 constexpr unsigned kPolls = 1u << 20;
 constexpr int kStatusWait = 64;
 
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
 #pragma unroll
                 for (int k = 0; k < 4; k++) { qb[nb][half * 4 + k][0] = r[2 * k]; qb[nb][half * 4 + k][1] = r[2 * k + 1]; }
             }
-        // sums in units of ref: [i][0], [1]: dim g * HD/8 + 2i of heads 2c, 2c + 1; [2], [3]: the next dim.  m, l: of heads 2c, 2c + 1
+        // sums in units of ref / kLift: [i][0], [1]: dim g * HD/8 + 2i of heads 2c, 2c + 1; [2], [3]: the next dim.  m, l: of heads 2c, 2c + 1
         float o[NB][MT][4], m[NB][2], l[NB][2], ref = 0.f;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
@@ -342,23 +342,28 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
         }
 
         // products of a tile (x[u]: tokens 16u + g, + 8) -> weights, with sc: bits of the exponent per unit of a product, and the sums so far
-        // brought to the new maximum
+        // brought to the new maximum.  Scores are rounded before the maximum is taken and subtracted, so that the largest weight is 1 whatever
+        // their size (rounded once after the difference, it would be up to 2^64 or down to 2^-64 with scores of 2^30).
         auto weigh = [&](float (&x)[NB][2][4], float sc0, float sc1) {
-            float shift[NB][2], fix[NB][2];
+            float at[NB][2], fix[NB][2];
             bool moved = false;
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][2 + e]) * sc0, fmaxf(x[nb][1][e], x[nb][1][2 + e]) * sc1);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        x[nb][u][e] = __fmul_rn(x[nb][u][e], u ? sc1 : sc0);
+                        x[nb][u][2 + e] = __fmul_rn(x[nb][u][2 + e], u ? sc1 : sc0);
+                    }
+                    float mx = fmaxf(fmaxf(x[nb][0][e], x[nb][0][2 + e]), fmaxf(x[nb][1][e], x[nb][1][2 + e]));
                     mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 8));
                     mx = fmaxf(m[nb][e], fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 16)));
-                    const float at = mx == -INFINITY ? 0.f : mx;
-                    fix[nb][e] = ex2(m[nb][e] - at);
+                    at[nb][e] = mx == -INFINITY ? 0.f : mx;
+                    fix[nb][e] = ex2(m[nb][e] - at[nb][e]);
                     moved |= mx != m[nb][e];
                     m[nb][e] = mx;
-                    shift[nb][e] = kLift - at;
                 }
             if (__any_sync(kFullMask, moved)) {
 #pragma unroll
@@ -377,11 +382,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        x[nb][u][e] = ex2(fmaf(x[nb][u][e], u ? sc1 : sc0, shift[nb][e & 1]));
+                        x[nb][u][e] = ex2(x[nb][u][e] - at[nb][e & 1]);
                         l[nb][e & 1] += x[nb][u][e];
                     }
         };
-        // brings the sums to a unit that is not below sv; the factor of weights whose values have the scale sv
+        // brings the sums to a unit that is not below sv; the factor of weights whose values have the scale sv, kLift in it
         auto unit_factor = [&](float sv) {
             if (sv > ref) {
                 const float f = ref / sv;
@@ -393,7 +398,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
                         for (int e = 0; e < 4; e++) o[nb][i][e] *= f;
                 ref = sv;
             }
-            return ref > 0.f ? __fdividef(sv, ref) : sv;
+            return (ref > 0.f ? __fdividef(sv, ref) : sv) * kLift;
         };
         // weights of 16 tokens, times f, as the second operand, in two parts of fp16: the second takes what the rounding of the first leaves.
         // (With one part the error of the result is 1.4 times that of its own rounding to fp16.)
@@ -548,7 +553,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[nb][i][e] *= ref;
+                for (int e = 0; e < 4; e++) o[nb][i][e] *= ref * (1.f / kLift);
         }
         const bool starts = w.t0 == 0, whole = starts && w.t1 == w.q.tiles;
         const int slot = 2 * blockIdx.x + (first ? 0 : 1);

@@ -367,6 +367,50 @@ def test_attention_not_finite():
         status.zero_()
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("gain", [100.0, 1e3, 1e4, 1.1e4, 1.3e4, 1.5e4, 2e4, 6e4])
+def test_attention_very_large_scores(gain, kind):
+    """Scores of 10^5 to 6 * 10^10 (128 products of gain * gain, / sqrt(128), in bits of the exponent): all weight on the token that looks where the
+    query does, or in equal parts on two of them, in blocks and in the tail; nothing overflows.  The weights are then 1, or 1/2 each, but for the two parts
+    of fp16 (2^-22) and the exponential's 2^-22; a value is off by the rounding to fp16 (2^-11 of itself, 2^-25 below 2^-14) and by 2^-20 of itself, far below the
+    2^-13 allowed here."""
+    kv, hd, block = 2, 128, 16
+    g = torch.Generator().manual_seed(int(gain))
+    places = [[3], [40, 150], [163], [5, 9], [161, 162], [0, 100]]           # of sequences of 165 tokens: ten blocks and five rows of the tail
+    S, n = len(places), 165
+    u = torch.where(torch.rand(kv, hd, generator=g) < 0.5, -1.0, 1.0)
+    c = R.Cache(S, S * 10, kv, hd, block, kind)
+    tables = torch.arange(S * 10, dtype=torch.int32).view(S, 10)
+    for s in range(S):
+        for t in range(n):
+            k = gain * u if t in places[s] else 0.01 * gain * torch.randn(kv, hd, generator=g)
+            c.append(s, t, k.half(), torch.randn(kv, hd, generator=g).half(), tables[s])
+    q = (gain * u).half().repeat_interleave(2, 0).view(1, -1).expand(S, -1).contiguous()
+    out, status = torch.zeros(S, 4 * hd, dtype=torch.float16, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.attn_decode_paged(out, q.to(DEV), *c.parts(DEV), tables.to(DEV), i32(*[n] * S).to(DEV), kind, status=status)
+    assert int(status) == 0
+    for s in range(S):
+        for h in range(4):
+            v = c.values(s, n, tables[s], h // 2, 1)[places[s]]
+            k = c.values(s, n, tables[s], h // 2, 0)[places[s]]
+            assert len(k) == 1 or torch.equal(k[0], k[1])                    # (of one size, in blocks too: the block's largest has its top code)
+            off = (out[s].cpu().double().view(4, hd)[h] - v.mean(0)).abs() - ((2.0 ** -11 + 2.0 ** -13) * v.abs().amax(0) + 2.0 ** -25)
+            assert float(off.max()) <= 0, (s, h, float(off.max()))
+
+
+def test_attention_keys_not_finite():
+    """A block whose keys stand for NaN, with finite values, makes its sequence and head NaN, no other."""
+    lengths, block = [64, 64], 32
+    c = random_cache(2, 4, 2, 64, block, "int8", 13)
+    tables = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 4 * 64).half().to(DEV)
+    good, out, parts = torch.empty_like(q), torch.empty_like(q), c.parts(DEV)
+    ops.attn_decode_paged(good, q, *parts, tables, i32(*lengths).to(DEV), "int8")
+    parts[1][1, 0, 0] = float("nan")
+    ops.attn_decode_paged(out, q, *parts, tables, i32(*lengths).to(DEV), "int8")
+    assert bool(out[0, :128].isnan().all()) and torch.equal(out[0, 128:], good[0, 128:]) and torch.equal(out[1], good[1])
+
+
 def test_attention_strides_streams_and_graph():
     """Rows inside wider buffers, tails inside a cache of several layers; two streams at once without a workspace; a captured call replayed with other
     lengths; the same bits each time."""

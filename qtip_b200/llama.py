@@ -518,6 +518,8 @@ class QtipLlama:
     def enable_beams(self, width, eos=-1):
         """The B rows of the batch become B / width groups of `width` beams (after enable_batch, before capture_batch).  feed_beams() takes the prompts,
         generate_batch() continues; then b_scores (groups, width) holds the sums of log probabilities, b_out_tokens the rows' tokens."""
+        if self.b_graph is not None:
+            raise RuntimeError("enable_beams() comes before capture_batch(): the captured step would go on sampling (release_graph() first)")
         assert 1 <= width <= ops.MAX_BEAMS and self.B % width == 0
         assert self.b_logits.shape[1] >= width, "fewer tokens than beams"
         G, dev = self.B // width, self.device

@@ -326,6 +326,20 @@ def test_beams_end():
     assert any(s == before[0] and t[2:] == [eos] * 6 for s, t in zip(scores, tokens))
 
 
+def test_beams_after_a_capture_are_refused():
+    """A captured step without beams would go on sampling: enable_beams() wants it released first."""
+    model = QtipLlama(SMALL, max_positions=32, device=DEV, seed=26)
+    model.enable_batch(2)
+    model.capture_batch()
+    with pytest.raises(RuntimeError, match="release_graph"):
+        model.enable_beams(2)
+    assert model.beam_width == 0
+    model.release_graph()
+    model.enable_beams(2)
+    model.feed_beams(torch.tensor([[1, 2]]))
+    assert bool(torch.isfinite(model.b_scores).all()) and bool((model.b_scores < 0).all())
+
+
 def test_pool_smaller_than_the_sequences():
     """A pool without room: the status says so, and the batch runs on with what it has."""
     model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=25)

@@ -553,11 +553,15 @@ class QtipLlama:
         self.b_pos.copy_(self.b_filled)
 
     def feed_beams(self, prompts):
-        """prompts (groups, n) token ids: every beam of a group takes its group's prompt; the last token's step is the first that selects."""
+        """prompts (groups, n) token ids: every beam of a group takes its group's prompt; the last token's step is the first that selects.  Begins a new
+        search: what an earlier one left is given up."""
         n = prompts.shape[1]
         assert prompts.shape[0] * self.beam_width == self.B and n >= 1
         if int(prompts.min()) < 0 or int(prompts.max()) >= self.shape.vocab:
             raise RuntimeError(f"a token outside the vocabulary of {self.shape.vocab}")
+        if n > self.max_positions:
+            raise RuntimeError(f"a prompt of {n} tokens: the KV cache holds {self.max_positions}")
+        self.reset_beams()
         self._reserve(n)
         rows = prompts.to(device=self.device, dtype=torch.int64).repeat_interleave(self.beam_width, 0)
         for i in range(n):

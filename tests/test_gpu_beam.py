@@ -340,6 +340,42 @@ def test_beams_after_a_capture_are_refused():
     assert bool(torch.isfinite(model.b_scores).all()) and bool((model.b_scores < 0).all())
 
 
+@pytest.mark.parametrize("kv", [None, "e4m3"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_second_search_starts_anew(kv, captured):
+    """feed_beams() after a finished search gives what a new model gives: tokens and scores, whatever the first search left in caches, tables and tails."""
+    prompts, found = [torch.tensor([[9, 8, 7, 6]]), torch.tensor([[400, 30]])], []
+    for searches in (prompts, prompts[1:]):
+        model = QtipLlama(SMALL, max_positions=32, device=DEV, seed=27)
+        model.enable_batch(3, kv=kv, block=16)
+        model.enable_beams(3)
+        if captured:
+            model.capture_batch()
+        for p in searches:
+            model.feed_beams(p)
+            model.generate_batch(21)
+        model.check_status()
+        assert model.b_pos.tolist() == [23] * 3
+        found.append((model.b_out_tokens[:, :24].clone(), model.b_scores.clone()))
+    assert torch.equal(found[0][0], found[1][0]) and torch.equal(found[0][1], found[1][1])
+
+
+def test_a_prompt_that_does_not_fit_is_refused():
+    """... and leaves the search as it was."""
+    model = QtipLlama(SMALL, max_positions=16, device=DEV, seed=29)
+    model.enable_batch(2)
+    model.enable_beams(2)
+    model.feed_beams(torch.tensor([[1, 2, 3]]))
+    before = model.b_scores.clone()
+    with pytest.raises(RuntimeError, match="holds 16"):
+        model.feed_beams(torch.zeros(1, 17, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        model.feed_beams(torch.full((1, 3), SMALL.vocab))
+    assert torch.equal(model.b_scores, before) and model.b_pos.tolist() == [3, 3] and model.steps_done == 3
+    with pytest.raises(RuntimeError, match="holds 16"):
+        model.generate_batch(14)
+
+
 def test_pool_smaller_than_the_sequences():
     """A pool without room: the status says so, and the batch runs on with what it has."""
     model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=25)

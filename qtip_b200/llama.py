@@ -526,6 +526,7 @@ class QtipLlama:
         self.beam_width, self.beam_eos = width, eos
         self.b_scores = torch.zeros(G, width, dtype=torch.float32, device=dev)
         self.b_parents = torch.zeros(G, width, dtype=torch.int32, device=dev)
+        self.b_last = torch.full((G, width), -1, dtype=torch.int64, device=dev)      # the tokens of the last selection: a prompt's own end nothing
         self.b_filled = torch.zeros(self.B, dtype=torch.int32, device=dev)
         log = (self.b_out_tokens.view(self.B, 1, -1, 1), 1, 0)
         if self.b_kv is None:
@@ -541,12 +542,12 @@ class QtipLlama:
         self.b_pos.zero_()
         self.b_scores.fill_(-math.inf)
         self.b_scores[:, 0] = 0.0
+        self.b_last.fill_(-1)
         self.steps_done = 0
 
     def _select_beams(self):
-        W = self.beam_width
-        tokens = self.b_token.view(-1, W)
-        ops.beam_select(tokens, self.b_parents, self.b_scores, self.b_logits, self.b_scores, tokens, self.beam_eos, status=self.status)
+        ops.beam_select(self.b_last, self.b_parents, self.b_scores, self.b_logits, self.b_scores, self.b_last, self.beam_eos, status=self.status)
+        self.b_token.copy_(self.b_last.view(-1))
         torch.add(self.b_pos, 1, out=self.b_filled)
         ops.beam_reorder(self.beam_states, self.b_parents, self.b_filled, status=self.status)
         self.b_out_tokens.scatter_(1, self.b_filled.long().view(-1, 1), self.b_token.view(-1, 1))

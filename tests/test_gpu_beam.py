@@ -376,6 +376,26 @@ def test_a_prompt_that_does_not_fit_is_refused():
         model.generate_batch(14)
 
 
+@pytest.mark.parametrize("prompts", [[[5, 6, 7], [300, 7, 7]], [[7], [7]]])
+@pytest.mark.parametrize("captured", [False, True])
+def test_prompts_that_hold_the_end_token(prompts, captured):
+    """The end token in a prompt ends nothing: the first selection is that of a search without an end, in a second search too."""
+    found = []
+    for eos in (-1, 7):
+        model = QtipLlama(SMALL, max_positions=32, device=DEV, seed=28)
+        model.enable_batch(6, kv="int8", block=16)
+        model.enable_beams(3, eos=eos)
+        if captured:
+            model.capture_batch()
+        for again in range(2):
+            model.feed_beams(torch.tensor(prompts))
+            found.append((model.b_token.clone(), model.b_scores.clone()))
+            model.generate_batch(2 if again == 0 else 0)
+        model.check_status()
+    for tokens, scores in found[1:]:
+        assert bool(torch.isfinite(scores).all()) and torch.equal(tokens, found[0][0]) and torch.equal(scores, found[0][1])
+
+
 def test_pool_smaller_than_the_sequences():
     """A pool without room: the status says so, and the batch runs on with what it has."""
     model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=25)

@@ -528,6 +528,7 @@ class QtipLlama:
         self.b_parents = torch.zeros(G, width, dtype=torch.int32, device=dev)
         self.b_last = torch.full((G, width), -1, dtype=torch.int64, device=dev)      # the tokens of the last selection: a prompt's own end nothing
         self.b_filled = torch.zeros(self.B, dtype=torch.int32, device=dev)
+        self.b_columns = torch.arange(self.max_positions + 1, dtype=torch.int32, device=dev)         # of the token log
         log = (self.b_out_tokens.view(self.B, 1, -1, 1), 1, 0)
         if self.b_kv is None:
             self.beam_states = [(self.b_cache_k, 1, 0), (self.b_cache_v, 1, 0), log]
@@ -550,7 +551,9 @@ class QtipLlama:
         self.b_token.copy_(self.b_last.view(-1))
         torch.add(self.b_pos, 1, out=self.b_filled)
         ops.beam_reorder(self.beam_states, self.b_parents, self.b_filled, status=self.status)
-        self.b_out_tokens.scatter_(1, self.b_filled.long().view(-1, 1), self.b_token.view(-1, 1))
+        # a comparison with every column instead of an index: steps behind the end of the log leave it as it is, and are reported
+        torch.where(self.b_columns == self.b_filled.view(-1, 1), self.b_token.view(-1, 1), self.b_out_tokens, out=self.b_out_tokens)
+        self.status.bitwise_or_((self.b_filled > self.max_positions).any() * 4)
         self.b_pos.copy_(self.b_filled)
 
     def feed_beams(self, prompts):

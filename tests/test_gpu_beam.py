@@ -396,6 +396,24 @@ def test_prompts_that_hold_the_end_token(prompts, captured):
         assert bool(torch.isfinite(scores).all()) and torch.equal(tokens, found[0][0]) and torch.equal(scores, found[0][1])
 
 
+@pytest.mark.parametrize("kv", [None, "int8"])
+def test_steps_behind_the_end_of_the_log(kv):
+    """step_batch() by hand, more often than there are positions: nothing is written behind the log, its rows stay the beams' tokens, the status says so."""
+    model = QtipLlama(SMALL, max_positions=16, device=DEV, seed=30)
+    model.enable_batch(2, kv=kv, block=16)
+    model.enable_beams(2)
+    for _ in range(16):
+        model.step_batch()
+    model.check_status()
+    rows = model.b_out_tokens.tolist()
+    for _ in range(5):
+        model.step_batch()
+    assert all(r in rows for r in model.b_out_tokens.tolist()) and model.b_pos.tolist() == [21, 21]
+    assert int(model.status) & 4
+    with pytest.raises(RuntimeError, match="4 = token log full"):
+        model.check_status()
+
+
 def test_pool_smaller_than_the_sequences():
     """A pool without room: the status says so, and the batch runs on with what it has."""
     model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=25)

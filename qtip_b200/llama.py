@@ -517,11 +517,14 @@ class QtipLlama:
     # -- beam search over the rows of the batch ---------------------------------------------------------
     def enable_beams(self, width, eos=-1):
         """The B rows of the batch become B / width groups of `width` beams (after enable_batch, before capture_batch).  feed_beams() takes the prompts,
-        generate_batch() continues; then b_scores (groups, width) holds the sums of log probabilities, b_out_tokens the rows' tokens."""
+        generate_batch() continues; then b_scores (groups, width) holds the sums of log probabilities, b_out_tokens the rows' tokens.  eos: the token
+        that ends a beam when a step chooses it (below 0: none)."""
         if self.b_graph is not None:
             raise RuntimeError("enable_beams() comes before capture_batch(): the captured step would go on sampling (release_graph() first)")
         assert 1 <= width <= ops.MAX_BEAMS and self.B % width == 0
         assert self.b_logits.shape[1] >= width, "fewer tokens than beams"
+        if eos >= self.shape.vocab:
+            raise RuntimeError(f"eos {eos} is outside the vocabulary of {self.shape.vocab}")
         G, dev = self.B // width, self.device
         self.beam_width, self.beam_eos = width, eos
         self.b_scores = torch.zeros(G, width, dtype=torch.float32, device=dev)

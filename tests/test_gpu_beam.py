@@ -414,6 +414,17 @@ def test_steps_behind_the_end_of_the_log(kv):
         model.check_status()
 
 
+def test_end_token_outside_the_vocabulary_is_refused():
+    """(Rows without a continuation take it as their next token.)"""
+    model = QtipLlama(SMALL, max_positions=16, device=DEV, seed=30)
+    model.enable_batch(2)
+    for eos in (SMALL.vocab, 1 << 40):
+        with pytest.raises(RuntimeError, match="outside the vocabulary"):
+            model.enable_beams(2, eos=eos)
+    assert model.beam_width == 0
+    model.enable_beams(2, eos=SMALL.vocab - 1)
+
+
 def test_pool_smaller_than_the_sequences():
     """A pool without room: the status says so, and the batch runs on with what it has."""
     model = QtipLlama(SMALL, max_positions=64, device=DEV, seed=25)

@@ -124,13 +124,30 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
             fresh = 0;
             len = max(len, 0);
         }
-        int need = in ? (len + fresh) / b - len / b : 0;
+        const int need = in ? (len + fresh) / b - len / b : 0;
         const int upto = block_scan(need, sums, total);
-        const long long base = base_at + upto - need;
-        base_at += total;
-        if (need > 0 && base + need > n_free) {              // the pool is exhausted
-            bad |= 8u;
-            fresh = need = 0;
+        long long base = base_at + upto - need;
+        if (base_at + total <= n_free) base_at += total;
+        else {
+            // The pool is exhausted: one sequence after the other, and one that does not fit takes nothing from those behind it.  (One thread; rare.)
+            s_base[tid] = need;
+            __syncthreads();
+            if (tid == 0) {
+                for (int i = 0; i < count; i++) {
+                    const int n = s_base[i];
+                    const bool fits = base_at + n <= n_free;
+                    s_base[i] = fits ? (int)base_at : -1;
+                    if (fits) base_at += n;
+                }
+                s_run[0] = (int)base_at;
+            }
+            __syncthreads();
+            base = s_base[tid];
+            base_at = s_run[0];
+            if (base < 0) {
+                bad |= 8u;
+                fresh = 0;
+            }
         }
         const int runs = fresh > 0 ? (len + fresh - 1) / b - len / b + 1 : 0;
         const int run = run_at + block_scan(runs, sums, total) - runs;

@@ -88,6 +88,46 @@ def test_plan_shares_and_releases():
     assert t.tolist() == [[0, 1, 2], [0, 1, 3], [4, -1, -1]] and out.tolist() == [48, 48, 16] and int(status) == 0
 
 
+@pytest.mark.parametrize("lengths, new, n_blocks, served", [
+    ([16, 15], [32, 1], 2, [16, 16]),                                      # needs of 2 and 1, one block free: the second is served
+    ([0, 0, 0, 0], [48, 16, 32, 16], 2, [0, 16, 0, 16]),
+    ([0, 31, 0, 7, 15], [15, 1, 200, 3, 1], 2, [15, 32, 0, 10, 15]),       # the second takes the one that is free, the last finds none
+    ([0, 31, 0, 7, 15], [15, 17, 200, 3, 1], 2, [15, 31, 0, 10, 16]),      # those that need no block are served too
+    ([0] * 1500, [16 + 16 * (i % 3) for i in range(1500)], 1004, None),
+    ([0] * 1200, [16] * 1023 + [48] + [16] * 176, 1025, None),             # across the 1024 sequences that are planned at a time
+    ([0] * 1200, [16] * 1000 + [48] * 24 + [32] * 176, 1001, None),
+    ([0] * 1200, [16] * 1000 + [48] * 24 + [32] * 100 + [16] * 76, 1001, None),
+])
+def test_plan_refused_sequences_take_nothing(lengths, new, n_blocks, served):
+    """Where the pool is exhausted, a sequence that does not fit is left out and takes no block from the ones behind it."""
+    block, S = 16, len(lengths)
+    tables = torch.full((S, 16), -1, dtype=torch.int32)
+    held = 0
+    for s, n in enumerate(lengths):
+        for j in range(n // block):
+            tables[s, j] = held
+            held += 1
+    free, want, out, names = n_blocks - held, 0, [], tables.clone()
+    for s in range(S):
+        need = (lengths[s] + new[s]) // block - lengths[s] // block
+        if want + need > free and need:
+            out.append(lengths[s])
+            continue
+        for j in range(need):
+            names[s, lengths[s] // block + j] = held + want + j
+        want += need
+        out.append(lengths[s] + new[s])
+    assert served is None or out == served
+    t, after, runs, n_runs, status = run_plan(tables, i32(*lengths), i32(*new), n_blocks, block, sum(new))
+    assert after.tolist() == out and torch.equal(t.cpu(), names) and int(status) == 8
+    first_row = [sum(new[:s]) for s in range(S)] if S < 10 else torch.tensor(new).cumsum(0).sub(torch.tensor(new)).tolist()
+    rows = runs[:int(n_runs)].tolist()
+    assert [r[0] for r in rows] == sorted(r[0] for r in rows) and sum(r[3] for r in rows) == sum(o - n for o, n in zip(out, lengths))
+    for seq, row, pos, count, b, _, _, _ in rows:
+        assert row == first_row[seq] + pos - lengths[seq] and out[seq] >= pos + count
+        assert b == (names[seq, pos // block] if (pos + count) % block == 0 else b) and ((pos + count) % block == 0 or b < 0)
+
+
 def test_plan_refusals():
     t, L = torch.zeros(2, 3, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
     out, runs, n = torch.zeros_like(L), torch.zeros(10, 8, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)

@@ -444,7 +444,8 @@ int qtip_kv_plan(int *tables, const int *lengths, const int *new_tokens, int *le
 
 /* Rotary embedding of q (n_tokens, n_heads * head_dim; to q_out, which may be q) and k, and append of k and v, along the runs of qtip_kv_plan.  Angle =
  * position * inv_freq[i] in 64 bits (inv_freq: head_dim/2 doubles), pairs (i, i + head_dim/2); the rotated k is rounded to fp16 before it is
- * stored or quantised.  Strides in elements between token rows (q, q_out, k, v) and sequences (tails); multiples of 8, pointers 16-byte aligned. */
+ * stored or quantised.  Strides in elements between token rows (q, q_out, k, v) and sequences (tails); multiples of 8, pointers 16-byte aligned;
+ * rows of q_out and tails of two sequences that overlap are refused. */
 int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const void *q, long q_stride, const void *k, long k_stride, const void *v,
                               long v_stride, void *data, float *scales, void *tail_k, long tail_k_stride, void *tail_v, long tail_v_stride,
                               const int *runs, const int *n_runs, int max_runs, const double *inv_freq, int n_tokens, int n_seqs, int n_heads,
@@ -453,7 +454,7 @@ int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const void *q, lon
 /* Single-query attention of each sequence over its lengths[s] cached tokens: out, q (n_seqs, n_heads * head_dim) fp16 with row strides; zeros for a
  * sequence without tokens.  A negative length or one that the table does not hold counts as 0 (status 1).  workspace:
  * qtip_attn_paged_workspace_bytes() bytes, no initialisation needed; not shared by calls that may overlap.  Strides multiples of 8 elements,
- * pointers 16-byte aligned. */
+ * pointers 16-byte aligned; rows of out that overlap are refused. */
 size_t qtip_attn_paged_workspace_bytes(int n_seqs, int n_heads, int n_kv_heads, int head_dim);
 int qtip_attn_decode_paged(void *out, long out_stride, const void *q, long q_stride, const void *data, const float *scales, const void *tail_k,
                            long tail_k_stride, const void *tail_v, long tail_v_stride, const int *tables, const int *lengths, int n_seqs,

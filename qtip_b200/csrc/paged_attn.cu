@@ -743,6 +743,7 @@ extern "C" int qtip_attn_decode_paged(void *out, long out_stride, const void *q,
         if (!aligned(p, 16)) return QTIP_ERR_ALIGNMENT;
     if (!aligned(tables, 4) || !aligned(lengths, 4) || !aligned(status, 4)) return QTIP_ERR_ALIGNMENT;
     if ((out_stride | q_stride | tail_k_stride | tail_v_stride) & 7) return QTIP_ERR_ALIGNMENT;
+    if (n_seqs > 1 && out_stride < (long)n_heads * head_dim) return QTIP_ERR_BAD_SHAPE;               // rows that are written share no memory
     uint8_t *w = static_cast<uint8_t *>(workspace);
     const AttnArgs a = {static_cast<__half *>(out), static_cast<const __half *>(q), out_stride, q_stride, static_cast<const uint8_t *>(data),
                         reinterpret_cast<const float4 *>(scales), static_cast<const __half *>(tail_k), static_cast<const __half *>(tail_v), tail_k_stride,

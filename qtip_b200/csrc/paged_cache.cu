@@ -467,6 +467,9 @@ extern "C" int qtip_rope_kv_append_paged(void *q_out, long q_out_stride, const v
         if (!aligned(p, 16)) return QTIP_ERR_ALIGNMENT;
     if (!aligned(inv_freq, 8) || !aligned(n_runs, 4) || !aligned(status, 4)) return QTIP_ERR_ALIGNMENT;
     if ((q_out_stride | q_stride | k_stride | v_stride | tail_k_stride | tail_v_stride) & 7) return QTIP_ERR_ALIGNMENT;
+    // rows that are written share no memory
+    const long tail = (long)n_kv_heads * block * head_dim;
+    if ((n_tokens > 1 && q_out_stride < (long)n_heads * head_dim) || (n_seqs > 1 && (tail_k_stride < tail || tail_v_stride < tail))) return QTIP_ERR_BAD_SHAPE;
     const AppendArgs a = {static_cast<__half *>(q_out), static_cast<const __half *>(q), static_cast<const __half *>(k), static_cast<const __half *>(v),
                           q_out_stride, q_stride, k_stride, v_stride, static_cast<uint8_t *>(data), reinterpret_cast<float4 *>(scales),
                           static_cast<__half *>(tail_k), static_cast<__half *>(tail_v), tail_k_stride, tail_v_stride, runs, n_runs, inv_freq, n_tokens,

@@ -567,3 +567,18 @@ def test_paged_refusals():
                         (0, q3[:, :128], "expected")):
         with pytest.raises(RuntimeError, match=match):
             ops.rope_kv_append_paged(*(fine[:i] + [v] + fine[i + 1:]))
+
+
+def test_output_rows_that_overlap_are_refused():
+    c = R.Cache(2, 4, 2, 64, 16, "int8")
+    parts = c.parts(DEV)
+    q, one = torch.zeros(2, 256, dtype=torch.float16, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    tables, L, runs = torch.zeros(2, 2, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(5, 8, dtype=torch.int32, device=DEV)
+    kv, freq = torch.zeros(2, 128, dtype=torch.float16, device=DEV), inv_freq(64).to(DEV)
+    for rows in (q[:1].expand(2, 256), q.view(-1).as_strided((2, 256), (128, 1))):
+        with pytest.raises(RuntimeError, match="shape"):
+            ops.attn_decode_paged(rows, q, *parts, tables, L, "int8")
+        with pytest.raises(RuntimeError, match="shape"):
+            ops.rope_kv_append_paged(rows, q, kv, kv, *parts, runs, one, freq, "int8")
+        ops.attn_decode_paged(torch.empty_like(q), rows, *parts, tables, L, "int8")                # read only: allowed
+    ops.attn_decode_paged(q[:1].expand(1, 256), q[:1], parts[0], parts[1], parts[2][:1], parts[3][:1], tables[:1], L[:1], "int8")

@@ -62,6 +62,18 @@ def test_attention_arguments():
     assert f(*(ok[:12] + [65535, 8, 2, 64, 1 << 20, 8, 16, 0, P, big, None, None])) == _lib.ERR_TOO_LARGE
 
 
+def test_rows_that_overlap_are_refused():
+    """Rows that are written: a stride below their width would have several CTAs write one place."""
+    lib = _lib.load()
+    append = [P, 128, P, 128, P, 64, P, 64, P, P, P, 1024, P, 1024, P, P, 4, P, 2, 2, 2, 1, 64, 4, 16, 0, None, None]
+    need = lib.qtip_attn_paged_workspace_bytes(2, 8, 2, 64)
+    attend = [P, 512, P, 512, P, P, P, 2048, P, 2048, P, P, 2, 8, 2, 64, 4, 8, 16, 0, P, need, None, None]
+    for f, ok, at, width in ((lib.qtip_rope_kv_append_paged, append, 1, 128), (lib.qtip_rope_kv_append_paged, append, 11, 1024),
+                             (lib.qtip_rope_kv_append_paged, append, 13, 1024), (lib.qtip_attn_decode_paged, attend, 1, 512)):
+        for stride in (0, 8, width - 8, -width):
+            assert f(*(ok[:at] + [stride] + ok[at + 1:])) == _lib.ERR_BAD_SHAPE, (at, stride)
+
+
 def test_beam_arguments():
     lib = _lib.load()
     ok = [P, P, P, P, _lib.F32, 100, P, P, 2, 4, 100, -1, None, None]

@@ -479,7 +479,8 @@ int qtip_beam_select(long long *tokens, int *parents, float *scores, const void 
  * (groups * width) sequences, seq_stride bytes apart, of `outer` pieces, outer_stride bytes apart, of `rows` rows of row_bytes (contiguous).
  * lengths (groups * width) or NULL: only rows below n / per_row, rounded up, are copied, n = the parent's length, modulo `mod` where mod > 0; rows
  * behind are left as they were.  Bytes and strides multiples of 4; faster at multiples of 16.  A parent outside the group: the row stays
- * (status 32).  At most 8 states in a call, which share no memory. */
+ * (status 32).  At most 8 states in a call, which share no memory; parents and lengths between a state's first and last
+ * byte are refused. */
 typedef struct qtip_beam_state {
     void *base;
     long seq_stride, outer_stride;

@@ -588,6 +588,15 @@ extern "C" int qtip_beam_reorder(const qtip_beam_state *states, int n_states, co
         ctas += (int)(want < most ? want : most);
     }
     if (width == 1) return QTIP_OK;
+    // every CTA reads these while others copy
+    const uintptr_t ints = 4u * (uintptr_t)groups * width;
+    for (int k = 0; k < n_states; k++) {
+        const qtip_beam_state &s = states[k];
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(s.base),
+                        hi = lo + ((uintptr_t)groups * width - 1) * s.seq_stride + (uintptr_t)(s.outer - 1) * s.outer_stride + (uintptr_t)s.rows * s.row_bytes;
+        for (const int *p : {parents, lengths})
+            if (p && reinterpret_cast<uintptr_t>(p) < hi && lo < reinterpret_cast<uintptr_t>(p) + ints) return QTIP_ERR_BAD_ARG;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, groups);
     cfg.blockDim = dim3(kReorderThreads);

@@ -218,6 +218,20 @@ def test_reorder_parents_outside_and_refusals():
         ops.beam_reorder(ok, torch.zeros(2, 2, dtype=torch.int32, device=DEV).t())
 
 
+def test_reorder_refuses_to_reorder_what_it_reads():
+    t, L = torch.arange(4 * 6, dtype=torch.int32, device=DEV).view(4, 1, 3, 2), torch.tensor([3, 2, 1, 0], dtype=torch.int32, device=DEV)
+    parents = torch.tensor([[1, 0, 3, 3]], dtype=torch.int32, device=DEV)
+    before = t.clone()
+    for states, p in (([(t, 1, 0), (L.view(4, 1, 1, 1), 1, 0)], parents), ([(t, 1, 0), (parents.view(4, 1, 1, 1), 1, 0)], parents)):
+        with pytest.raises(RuntimeError, match="bad argument"):
+            ops.beam_reorder(states, p, L)
+    assert torch.equal(t, before)
+    both = torch.cat([parents.view(-1), L, t.view(-1)])                   # beside one another: allowed
+    live = both[8:].view(4, 1, 3, 2)
+    ops.beam_reorder([(live, 1, 0)], both[:4].view(1, 4), both[4:8])
+    assert torch.equal(live, reordered(before, parents, L, 1, 0)) and torch.equal(both[:8], torch.cat([parents.view(-1), L]))
+
+
 # ------------------------------------------------------------------------------------------------------------ in the model
 SMALL = LlamaShape(n_layers=2, hidden=512, n_heads=4, n_kv_heads=2, head_dim=128, mlp=1376, vocab=700, K=2)
 

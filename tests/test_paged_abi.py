@@ -105,6 +105,22 @@ def test_beam_arguments():
     assert reorder(width=1) == _lib.OK                            # a beam alone has nowhere to go
 
 
+def test_reorder_refuses_to_reorder_what_it_reads():
+    """Parents or lengths inside a state: some CTAs would read them before, others after the copy."""
+    f = _lib.load().qtip_beam_reorder
+
+    def st(base, parents, lengths, n=1, **kw):
+        state = dict(dict(seq_stride=8, outer_stride=8, outer=1, rows=1, row_bytes=4, per_row=1, mod=0), **kw)
+        states = [_lib.BeamState(base=P + 2048, **state), _lib.BeamState(base=base, **state)][2 - n:]
+        return f((_lib.BeamState * n)(*states), n, parents, lengths, 2, 2, None, None)
+    # 2 groups of 2: 16 bytes of either; a state of 4 sequences, 8 bytes apart: 28 bytes
+    for at in (P + 1024, P + 1024 - 12, P + 1024 + 24, P + 1024 + 8):
+        for n in (1, 2):
+            assert st(P + 1024, at, None, n) == _lib.ERR_BAD_ARG and st(P + 1024, P, at, n) == _lib.ERR_BAD_ARG
+    assert st(P + 1024, P, P + 1024 + 40, outer=2, seq_stride=24, outer_stride=12) == _lib.ERR_BAD_ARG
+    assert st(P + 1024, P + 1024, None, rows=0) == _lib.ERR_BAD_SHAPE
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_places_in_a_unit(hd):
     for which in (0, 1):

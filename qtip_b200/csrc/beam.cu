@@ -1,5 +1,7 @@
 // Beam search: the selection of each group's best continuations, and the reordering of what belongs to a beam (caches, block tables,
 // token logs).  They stand where the decode loop samples (eval/interactive_gen.py:15-40 upstream).
+#include <atomic>
+
 #include "common.cuh"
 
 namespace qtip {
@@ -499,7 +501,8 @@ constexpr size_t select_smem_bytes() {
 // 74 us with 4 and 60 with 8; one group 28 us with 8 and 21 with 16 (where the GPU has room for clusters of 16).
 template <typename T>
 int launch_select(const SelectArgs &a, int groups, cudaStream_t stream) {
-    static int cached[64][5] = {};       // clusters of 1, 2, 4, 8, 16 CTAs at once, plus one
+    // clusters of 1, 2, 4, 8, 16 CTAs at once, plus one; filled by whichever thread comes first, after it has set what a launch of that size needs
+    static std::atomic<int> cached[64][5] = {};
     int dev = 0, cluster = 0;
     QTIP_CUDA_TRY(cudaGetDevice(&dev));
     QTIP_CUDA_TRY(cudaFuncSetAttribute(beam_select_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)select_smem_bytes<T>()));
@@ -517,7 +520,7 @@ int launch_select(const SelectArgs &a, int groups, cudaStream_t stream) {
     for (int k = 0; k < 5; k++) {
         const int c = 1 << k, per = c * (kSelectThreads / 32) / a.width;                   // warps of a row
         if (per == 0) continue;
-        int n = dev < 64 ? cached[dev][k] - 1 : -1;
+        int n = dev < 64 ? cached[dev][k].load(std::memory_order_acquire) - 1 : -1;
         if (n < 0) {
             cfg.gridDim = dim3(c);
             cfg.numAttrs = 1;
@@ -527,7 +530,7 @@ int launch_select(const SelectArgs &a, int groups, cudaStream_t stream) {
                 (void)cudaGetLastError();
                 n = 0;
             }
-            if (dev < 64) cached[dev][k] = n + 1;
+            if (dev < 64) cached[dev][k].store(n + 1, std::memory_order_release);
         }
         if (c == 16 && n < groups) continue;
         const double time = n ? (double)((groups + n - 1) / n) / per : 1e30;               // rounds, each as long as a warp's part of a row

@@ -132,6 +132,35 @@ def test_select_fewer_tokens_than_beams():
     check_select(torch.randn(12, 4, generator=torch.Generator().manual_seed(8)), scores)
 
 
+def test_select_from_several_threads():
+    """The C entry from four threads at once, on streams of their own, with widths and numbers of groups that take different clusters."""
+    import threading
+
+    from qtip_b200 import _lib
+    lib, cases = _lib.load(), []
+    for W, G, V in ((1, 1, 4001), (4, 3, 2000), (16, 1, 9000), (8, 40, 700)):
+        logits, scores = torch.randn(G * W, V, generator=torch.Generator().manual_seed(W)).to(DEV), torch.zeros(G, W, device=DEV)
+        want = select(logits, scores, None, -1)
+        out = [torch.zeros(G, W, dtype=torch.int64, device=DEV), torch.zeros(G, W, dtype=torch.int32, device=DEV), torch.zeros(G, W, device=DEV)]
+        cases.append((W, G, V, logits, scores, want, out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    codes = []
+
+    def run(W, G, V, logits, scores, want, out, stream):
+        for _ in range(50):
+            codes.append(lib.qtip_beam_select(*(t.data_ptr() for t in out), logits.data_ptr(), _lib.F32, V, scores.data_ptr(), None, G, W, V, -1, None,
+                                              stream.cuda_stream))
+    threads = [threading.Thread(target=run, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [0] * 200
+    for c in cases:
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(c[6], c[5]))
+
+
 def test_select_refusals():
     G, W, V = 2, 4, 50
     z = lambda dt: torch.zeros(G, W, dtype=dt, device=DEV)  # noqa: E731

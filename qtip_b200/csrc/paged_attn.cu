@@ -1,7 +1,8 @@
 // Single-query attention over the key/value cache in 8 bits (paged.cuh): out = softmax(q K^T / sqrt(hd)) V for each sequence and head.
 // Stands where the decode loop has the scaled_dot_product_attention of LlamaSdpaAttention.forward (model/llama.py:884-891 upstream).
 //
-// Bound by the bytes of the cache: 2 per token, key/value head and dim, read once for all query heads that share them.
+// Bound by the bytes of the cache: 2 per token, key/value head and dim, read once for up to 16 query heads that share them (their scores and sums fill a
+// warp's registers), twice for 17 to 32, and so on.
 // A pair is a sequence and a key/value head (of at most 16 query heads; more are further pairs).  Its tokens are cut into tiles of 32, and the
 // tiles of all pairs, in order, are dealt to the CTAs in equal contiguous ranges, computed by every CTA from the lengths: a long sequence is
 // spread over the chip, and a CTA goes through several short ones.  The start of a pair counts as kStart tiles (its queries, and the join of the
@@ -141,6 +142,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<HD, NB>::kCtas) attn_p
     float *join = reinterpret_cast<float *>(ring_scale + kAttnWarps * kStages * 2);       // [warp][kJoin][32]
     float2 *join_ml = reinterpret_cast<float2 *>(join + kAttnWarps * kJoin * 32);         // [warp][head of 8 NB]
     __shared__ uint64_t bars[kAttnWarps][kStages];
+    // The ranges are cut for kCtas per SM.  Registers are held to that by the launch bounds, shared memory (228 KB per SM, in steps of 128 bytes, 1 KB of it
+    // the system's for each CTA; for 128 dims and 16 query heads it is used to the last byte) by this.
+    static_assert(Shape::kCtas * ((Shape::kSmem + sizeof(bars) + 127) / 128 * 128 + 1024) <= 228 * 1024, "an SM does not hold kCtas of these CTAs");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, sh = a.shift, b = 1 << sh;
     const int pairs = a.n_kv * a.groups;                                                  // of a sequence
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -335,6 +335,77 @@ def test_attention_split(lengths, heads, kv, hd, block, kind):
     check_attention(c, lengths, tables_for(lengths, block, n_blocks, max(lengths) // block + 1), heads)
 
 
+def marked_cache(S, n_blocks, kv, hd, block, kind, seed):
+    """A pool in which block j's values are one number, different from block to block, in dim j of 64 (and 64 + j), zero elsewhere: a dim of the result is the
+    weight of the tokens whose blocks carry it, so a tile that is left out or counted twice shows."""
+    c = random_cache(S, n_blocks, kv, hd, block, kind, seed)
+    one = torch.full((block, hd), 128 if kind == "int8" else 0, dtype=torch.uint8)
+    for j in range(n_blocks):
+        codes = one.clone()
+        codes[:, [d for d in range(hd) if d % 64 == j % 64]] = 255 if kind == "int8" else 0x7E          # the largest value
+        c.data[j, :, :, 1] = R.pack(codes, 1)
+        c.scales[j, :, 1] = (1 + j % 7 / 8) / R.TOP[kind]
+    c.tail_v = c.tail_v.abs()
+    return c
+
+
+def sections(lengths, block, n_blocks, mb, tokens):
+    """Tables in which consecutive stretches of `tokens` tokens name one block."""
+    t = torch.full((len(lengths), mb), 1 << 30, dtype=torch.int32)
+    for s, n in enumerate(lengths):
+        t[s, :n // block] = ((torch.arange(n // block) * block // tokens * 5 + s) % n_blocks).int()
+    return t
+
+
+def check_marked(c, lengths, heads, tokens):
+    """All values are at least 0, so every sum keeps its relative error: half a step of the result (2^-11); scores of below 2^4 bits, off by 2^-19 in fp32, with
+    the exponential's and the two parts' 2^-22: 2^-18 in a weight; up to 2^9 additions of a lane and 2^9 of the parts at 2^-24 to 2^-23 each: 2^-13."""
+    mb = max(lengths) // c.block
+    tables = sections(lengths, c.block, c.data.shape[0], max(mb, 1), tokens)
+    q = torch.randn(len(lengths), heads * c.hd, generator=torch.Generator().manual_seed(3)).mul(0.5).half().to(DEV)
+    out, status = torch.full_like(q, 7.0), torch.zeros(1, dtype=torch.int32, device=DEV)
+    parts = c.parts(DEV)
+    ops.attn_decode_paged(out, q, *parts, tables.to(DEV), i32(*lengths).to(DEV), c.kind, status=status)
+    assert int(status) == 0
+    rep, lut = heads // c.kv, R.code_values(c.kind).to(DEV)
+    for s, n in enumerate(lengths):
+        got = out[s].double().view(heads, c.hd)
+        if n == 0:
+            assert bool((got == 0).all())
+            continue
+        ids = tables[s, :n // c.block].long().to(DEV)
+        for h in range(c.kv):
+            kv = []
+            for w, tail in ((0, parts[2][s, h]), (1, parts[3][s, h].permute(0, 2, 1).reshape(c.block, c.hd))):
+                pool = lut[parts[0][:, h, :, w][..., R.places(w, c.hd).to(DEV)].long()].view(-1, c.block, c.hd) * parts[1][:, h, w].double()[:, None, None]
+                kv.append(torch.cat([pool[ids].reshape(-1, c.hd), tail[:n % c.block].double()]))
+            p = torch.softmax(q[s].view(heads, c.hd)[h * rep:(h + 1) * rep].double() @ kv[0].T / math.sqrt(c.hd), 1)
+            want = p @ kv[1]
+            off = (got[h * rep:(h + 1) * rep] - want).abs() - ((2.0 ** -11 + 2.0 ** -12) * want + 2.0 ** -25)
+            assert float(off.max()) <= 0, (s, n, h, float(off.max()), float(want.max()))
+
+
+@pytest.mark.parametrize("heads, kv, hd, block, kind, lengths", [
+    (4, 4, 128, 16, "int8", [40001, 0, 131071, 7, 90000, 1, 200016, 33333, 131072]),           # up to 8 query heads on one, 128 dims: from 71040 tiles
+    (32, 2, 128, 32, "e4m3", [300033, 1000, 0, 262144, 129, 250001]),                           # 16 of them: from 47360
+    (17, 1, 64, 64, "int8", [700001, 0, 450000, 64, 500063]),                                   # two groups, 64 dims: from 94720
+    (4, 2, 64, 16, "e4m3", [500001, 1000, 0, 262144, 15, 850001, 31, 750016]),                  # 64 dims: from 142080
+])
+def test_attention_ranges_in_waves(heads, kv, hd, block, kind, lengths):
+    """So many tiles that the CTAs take them in waves of smaller ranges; pairs that cross from one wave into the next; sequences of none between."""
+    groups = -(-heads // kv // 16)
+    tiles = sum((n // block * block + 31) // 32 + (n % block + 15) // 16 + 4 for n in lengths if n) * kv * groups
+    ctas = torch.cuda.get_device_properties(0).multi_processor_count * (3 if heads // kv <= 8 else 2)
+    assert tiles >= ctas * (160 if hd == 128 else 320)
+    check_marked(marked_cache(len(lengths), 67, kv, hd, block, kind, 31), lengths, heads, 2000)
+
+
+@pytest.mark.parametrize("heads, hd, kind", [(4, 128, "int8"), (16, 128, "e4m3"), (1, 64, "int8")])
+def test_attention_joins_many_parts(heads, hd, kind):
+    """A pair in more than 256 parts (a CTA's threads): the join goes through them in steps, with what it has so far carried on."""
+    check_marked(marked_cache(2, 67, 1, hd, 64, kind, 32), [131071, 5], heads, 512)
+
+
 @pytest.mark.parametrize("gain", [0.0, 30.0])
 def test_attention_flat_and_peaked(gain):
     """All scores equal; one score far above the others (scores of some hundreds: their fp32 sums are off by 2^-14, the allowance for weights holds as

@@ -530,7 +530,6 @@ class QtipLlama:
         self.b_scores = torch.zeros(G, width, dtype=torch.float32, device=dev)
         self.b_parents = torch.zeros(G, width, dtype=torch.int32, device=dev)
         self.b_last = torch.full((G, width), -1, dtype=torch.int64, device=dev)      # the tokens of the last selection: a prompt's own end nothing
-        self.b_filled = torch.zeros(self.B, dtype=torch.int32, device=dev)
         self.b_columns = torch.arange(self.max_positions + 1, dtype=torch.int32, device=dev)         # of the token log
         log = (self.b_out_tokens.view(self.B, 1, -1, 1), 1, 0)
         if self.b_kv is None:
@@ -552,12 +551,11 @@ class QtipLlama:
     def _select_beams(self):
         ops.beam_select(self.b_last, self.b_parents, self.b_scores, self.b_logits, self.b_scores, self.b_last, self.beam_eos, status=self.status)
         self.b_token.copy_(self.b_last.view(-1))
-        torch.add(self.b_pos, 1, out=self.b_filled)
-        ops.beam_reorder(self.beam_states, self.b_parents, self.b_filled, status=self.status)
+        self.b_pos.add_(1)
+        ops.beam_reorder(self.beam_states, self.b_parents, self.b_pos, status=self.status)
         # a comparison with every column instead of an index: steps behind the end of the log leave it as it is, and are reported
-        torch.where(self.b_columns == self.b_filled.view(-1, 1), self.b_token.view(-1, 1), self.b_out_tokens, out=self.b_out_tokens)
-        self.status.bitwise_or_((self.b_filled > self.max_positions).any() * 4)
-        self.b_pos.copy_(self.b_filled)
+        torch.where(self.b_columns == self.b_pos.view(-1, 1), self.b_token.view(-1, 1), self.b_out_tokens, out=self.b_out_tokens)
+        self.status.bitwise_or_((self.b_pos > self.max_positions).any() * 4)
 
     def feed_beams(self, prompts):
         """prompts (groups, n) token ids: every beam of a group takes its group's prompt; the last token's step is the first that selects.  Begins a new

@@ -423,7 +423,8 @@ int qtip_attn_decode_batch(void *out, const void *q, const void *cache_k, const 
  *   tail_k  (n_seqs, n_kv_heads, block, head_dim) fp16, tail_v (n_seqs, n_kv_heads, block/2, head_dim, 2) fp16 (pairs of tokens), any stride
  *           between sequences
  * QTIP_KV_INT8: value = (byte - 128) * scale, scale = largest magnitude / 127; QTIP_KV_E4M3: value = e4m3 * scale, scale = largest / 448
- * (the largest is at least 2^-24).  A block in which some value is not finite has the scale NaN: all its tokens stand for NaN.
+ * (the largest is at least 2^-24).  A block in which some value is not finite has the scale NaN: all its tokens stand for NaN.  In the tail
+ * values are what they are; one of V that is not finite leaves its dim of the attention's result not finite (NaN or infinity), the others as they are.
  * head_dim 64 or 128.  All follow stream order for every operand.  `status` (optional) as for the decode loop, and 8: the pool is exhausted,
  * 16: a table names no block of the pool (attention: the sequence's result is NaN), 32: a beam's parent outside its group, 64: a bounded wait of
  * the attention for its own copies ran out (results are meaningless, the kernel ends).

@@ -13,8 +13,8 @@ namespace {
 // list to keep, a sequence whose length is set to zero has released its blocks, and tables that name the same block (beams of one
 // search, a common prompt) share it.  The new blocks are the lowest free ones, in the order of the sequences.
 // One CTA; for many table entries a cluster of eight, each of which marks every eighth share of 32 sequences in a bitmap of its own, which the first
-// then takes over (marking is bound by the shared-memory atomics of an SM: 512 sequences with 130000 blocks 31 us with one CTA, 18 with
-// eight; eight sequences of at most 128 blocks 5.4 with one).
+// then takes over: marking is bound by the shared-memory atomics of an SM.  With one CTA and with eight, tables of n entries, all but a few in
+// use: 1024 entries 4.6 and 5.5 us, 8192 6.0 and 6.6, 16384 7.2 and 7.0, 32768 9.4 and 7.5, 65536 13.7 and 8.7, 262144 34 and 16.
 constexpr int kPlanThreads = 1024, kPlanLoads = 8, kPlanCluster = 8, kPlanEntries = 32768, kPlanMaxBlocks = 1600000, kPlanMaxTokens = 1 << 20;
 
 struct PlanArgs {

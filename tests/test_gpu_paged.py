@@ -522,6 +522,25 @@ def test_attention_keys_not_finite():
     assert bool(out[0, :128].isnan().all()) and torch.equal(out[0, 128:], good[0, 128:]) and torch.equal(out[1], good[1])
 
 
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_attention_values_not_finite_in_the_tail(value):
+    """Their dim is not finite, the other dims and the other heads are what they would be."""
+    lengths, block = [70], 32
+    c = random_cache(1, 2, 2, 64, block, "int8", 14)
+    tables = torch.tensor([[0, 1]], dtype=torch.int32)
+    q = torch.randn(1, 4 * 64, generator=torch.Generator().manual_seed(5)).half()
+    out = torch.zeros(1, 4 * 64, dtype=torch.float16, device=DEV)
+    want = c.attend(q.view(4, 64), 0, 70, tables[0])
+    top = float(max(c.values(0, 70, tables[0], h, 1).abs().max() for h in range(2)))
+    c.tail_v[0, 1, 2, 17, 1] = value                         # token 69, key/value head 1, dim 17
+    ops.attn_decode_paged(out, q.to(DEV), *c.parts(DEV), tables.to(DEV), i32(*lengths).to(DEV), "int8")
+    out = out.cpu().view(4, 64).double()
+    assert not bool(torch.isfinite(out[2:, 17]).any())
+    out[2:, 17] = want[2:, 17]
+    # as check_attention: half a step of fp16 and 2^-15 of the largest value
+    assert float(((out - want).abs() - (2.0 ** -11 * want.abs() + 2.0 ** -15 * top + 2.0 ** -25)).max()) <= 0
+
+
 def test_attention_strides_streams_and_graph():
     """Rows inside wider buffers, tails inside a cache of several layers; two streams at once without a workspace; a captured call replayed with other
     lengths; the same bits each time."""

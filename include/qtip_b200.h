@@ -438,8 +438,8 @@ enum { QTIP_KV_INT8 = 0, QTIP_KV_E4M3 = 1 };
  * first token row, first position, tokens, pool block (-1: stays in the tail; -2: in the tail, written with the sequence's first run), for
  * that first run the number of this one else -1, 0, 0; n_runs their number; rows of `runs` behind it are left as they were.
  * A sequence that cannot be served (negative numbers, more than max_blocks complete blocks, rows behind n_tokens: status 1; more blocks than the ones before it
- * left free: status 8) keeps its length (0 for a negative one), gets no run and takes no block from those behind it.  max_runs >= n_tokens / block + 2 * n_seqs.  runs 16-byte aligned; n_blocks <= 1600000,
- * n_tokens <= 2^20, positions below 2^31. */
+ * left free: status 8) keeps its length (0 for a negative one), gets no run and takes no block from those behind it.
+ * max_runs >= n_tokens / block + 2 * n_seqs.  runs 16-byte aligned; n_blocks <= 1600000, n_tokens <= 2^20, positions below 2^31. */
 int qtip_kv_plan(int *tables, const int *lengths, const int *new_tokens, int *lengths_out, int *runs, int *n_runs, int n_seqs, int max_blocks,
                  int n_blocks, int block, int n_tokens, int max_runs, unsigned *status, void *stream);
 

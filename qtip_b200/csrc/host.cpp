@@ -350,6 +350,11 @@ long rows_of(const char *name, const at::Tensor &t, int64_t rows, int64_t width)
     if (width > 1 && t.stride(1) != 1) throw Failure{std::string(name) + ": the values of a row have to be contiguous"};
     return rows > 1 ? t.stride(0) : width;
 }
+// The library counts in 32 bits: a size or number beyond them must not come out as another one.
+int narrow(const char *name, int64_t v) {
+    if (v < INT32_MIN || v > INT32_MAX) throw Failure{std::string(name) + " is out of range: " + std::to_string(v)};
+    return (int)v;
+}
 void *current_stream() { return at::cuda::getCurrentCUDAStream(c10::cuda::current_device()).stream(); }
 unsigned *status_of(const at::Tensor *t) {
     if (!t) return nullptr;
@@ -376,6 +381,11 @@ struct KvCache {
             throw Failure{"the tails of one sequence have to be contiguous"};
         if (seqs > 1 && (tail_k.stride(0) < kv * block * hd || tail_v.stride(0) < kv * block * hd)) throw Failure{"the tails of two sequences overlap"};
     }
+    int n_seqs() const { return narrow("n_seqs", seqs); }
+    int n_blocks() const { return narrow("n_blocks", blocks); }
+    int n_kv() const { return narrow("n_kv", kv); }
+    int head_dim() const { return narrow("head_dim", hd); }
+    int block_size() const { return narrow("block", block); }
     long stride_k() const { return seqs > 1 ? tail_k.stride(0) : 0; }
     long stride_v() const { return seqs > 1 ? tail_v.stride(0) : 0; }
     const at::Tensor *list[4] = {&data, &scales, &tail_k, &tail_v};
@@ -404,10 +414,10 @@ PyObject *py_kv_plan(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         expect("lengths_out", lengths_out, at::kInt, {S});
         expect("runs", runs, at::kInt, {runs.size(0), 8});
         expect("n_runs", n_runs, at::kInt, {1});
-        if (n_blocks > INT32_MAX || n_tokens > INT32_MAX || block > INT32_MAX) throw Failure{"n_blocks, block, n_tokens: 32-bit numbers expected"};
         check(qtip_kv_plan(static_cast<int *>(tables.data_ptr()), static_cast<const int *>(lengths.data_ptr()), static_cast<const int *>(fresh.data_ptr()),
-                           static_cast<int *>(lengths_out.data_ptr()), static_cast<int *>(runs.data_ptr()), static_cast<int *>(n_runs.data_ptr()), (int)S,
-                           (int)tables.size(1), (int)n_blocks, (int)block, (int)n_tokens, (int)std::min<int64_t>(runs.size(0), INT32_MAX), status_of(status),
+                           static_cast<int *>(lengths_out.data_ptr()), static_cast<int *>(runs.data_ptr()), static_cast<int *>(n_runs.data_ptr()), narrow("n_seqs", S),
+                           narrow("max_blocks", tables.size(1)), narrow("n_blocks", n_blocks), narrow("block", block), narrow("n_tokens", n_tokens),
+                           (int)std::min<int64_t>(runs.size(0), INT32_MAX), status_of(status),
                            current_stream()),
               "qtip_kv_plan");
         return 1L;
@@ -427,12 +437,11 @@ PyObject *py_rope_kv_append_paged(PyObject *, PyObject *const *a, Py_ssize_t nar
         expect("inv_freq", inv_freq, at::kDouble, {c.hd / 2});
         if (width % c.hd) throw Failure{"q: a multiple of head_dim values in a row expected"};
         const long sqo = rows_of("q_out", q_out, T, width), sq = rows_of("q", q, T, width), sk = rows_of("k", k, T, c.kv * c.hd), sv = rows_of("v", v, T, c.kv * c.hd);
-        if (T > INT32_MAX || c.blocks > INT32_MAX) throw Failure{"too many token rows or blocks"};
         check(qtip_rope_kv_append_paged(q_out.data_ptr(), sqo, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, c.data.data_ptr(),
                                         static_cast<float *>(c.scales.data_ptr()), c.tail_k.data_ptr(), c.stride_k(), c.tail_v.data_ptr(), c.stride_v(),
                                         static_cast<const int *>(runs.data_ptr()), static_cast<const int *>(n_runs.data_ptr()),
-                                        (int)std::min<int64_t>(runs.size(0), INT32_MAX), static_cast<const double *>(inv_freq.data_ptr()), (int)T,
-                                        (int)c.seqs, (int)(width / c.hd), (int)c.kv, (int)c.hd, (int)c.blocks, (int)c.block, (int)int_arg(a[11]),
+                                        (int)std::min<int64_t>(runs.size(0), INT32_MAX), static_cast<const double *>(inv_freq.data_ptr()), narrow("n_tokens", T),
+                                        c.n_seqs(), narrow("n_heads", width / c.hd), c.n_kv(), c.head_dim(), c.n_blocks(), c.block_size(), narrow("kind", int_arg(a[11])),
                                         status_of(status), current_stream()),
               "qtip_rope_kv_append_paged");
         return 1L;
@@ -451,17 +460,17 @@ PyObject *py_attn_decode_paged(PyObject *, PyObject *const *a, Py_ssize_t nargs)
         expect("tables", tables, at::kInt, {c.seqs, tables.size(1)});
         expect("lengths", lengths, at::kInt, {c.seqs});
         const long so = rows_of("out", out, c.seqs, width), sq = rows_of("q", q, c.seqs, width);
-        if (n_heads > INT32_MAX || c.blocks > INT32_MAX || tables.size(1) > INT32_MAX) throw Failure{"too many heads or blocks"};
+        const int heads = narrow("n_heads", n_heads);
         at::Tensor own;                  // from torch's allocator: of the stream, or of the graph that is being captured
         if (!workspace) {
-            const size_t need = qtip_attn_paged_workspace_bytes((int)c.seqs, (int)n_heads, (int)c.kv, (int)c.hd);
+            const size_t need = qtip_attn_paged_workspace_bytes(c.n_seqs(), heads, c.n_kv(), c.head_dim());
             own = at::empty({(int64_t)std::max<size_t>(need, 1)}, q.options().dtype(at::kByte));
             workspace = &own;
         }
         check(qtip_attn_decode_paged(out.data_ptr(), so, q.data_ptr(), sq, c.data.data_ptr(), static_cast<const float *>(c.scales.data_ptr()),
                                      c.tail_k.data_ptr(), c.stride_k(), c.tail_v.data_ptr(), c.stride_v(), static_cast<const int *>(tables.data_ptr()),
-                                     static_cast<const int *>(lengths.data_ptr()), (int)c.seqs, (int)n_heads, (int)c.kv, (int)c.hd, (int)tables.size(1),
-                                     (int)c.blocks, (int)c.block, (int)int_arg(a[8]), workspace->data_ptr(), workspace->nbytes(), status_of(status),
+                                     static_cast<const int *>(lengths.data_ptr()), c.n_seqs(), heads, c.n_kv(), c.head_dim(), narrow("max_blocks", tables.size(1)),
+                                     c.n_blocks(), c.block_size(), narrow("kind", int_arg(a[8])), workspace->data_ptr(), workspace->nbytes(), status_of(status),
                                      current_stream()),
               "qtip_attn_decode_paged");
         return 1L;
@@ -483,10 +492,9 @@ PyObject *py_beam_select(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
         if (logits.size(0) != G * W || (vocab > 1 && logits.stride(1) != 1)) throw Failure{"logits: (groups * width, vocab) with contiguous rows expected, not " + text(logits.sizes())};
         const long long eos = PyLong_AsLongLong(a[6]);
         if (eos == -1 && PyErr_Occurred()) throw Failure{""};
-        if (vocab > INT32_MAX) throw Failure{"too large a vocabulary"};
         check(qtip_beam_select(reinterpret_cast<long long *>(tokens.data_ptr()), static_cast<int *>(parents.data_ptr()), static_cast<float *>(scores.data_ptr()),
                                logits.data_ptr(), dtype_id(logits), G * W > 1 ? logits.stride(0) : vocab, static_cast<const float *>(prev_scores.data_ptr()),
-                               prev_tokens ? reinterpret_cast<const long long *>(prev_tokens->data_ptr()) : nullptr, (int)G, (int)W, (int)vocab, eos,
+                               prev_tokens ? reinterpret_cast<const long long *>(prev_tokens->data_ptr()) : nullptr, narrow("groups", G), narrow("width", W), narrow("vocab", vocab), eos,
                                status_of(status), current_stream()),
               "qtip_beam_select");
         return 1L;
@@ -526,7 +534,7 @@ PyObject *py_beam_reorder(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
             list[i].mod = (int)mod;
         }
         check(qtip_beam_reorder(list, (int)n, static_cast<const int *>(parents.data_ptr()), lengths ? static_cast<const int *>(lengths->data_ptr()) : nullptr,
-                                (int)G, (int)W, status_of(status), current_stream()),
+                                narrow("groups", G), narrow("width", W), status_of(status), current_stream()),
               "qtip_beam_reorder");
         return 1L;
     });

@@ -672,3 +672,22 @@ def test_output_rows_that_overlap_are_refused():
             ops.rope_kv_append_paged(rows, q, kv, kv, *parts, runs, one, freq, "int8")
         ops.attn_decode_paged(torch.empty_like(q), rows, *parts, tables, L, "int8")                # read only: allowed
     ops.attn_decode_paged(q[:1].expand(1, 256), q[:1], parts[0], parts[1], parts[2][:1], parts[3][:1], tables[:1], L[:1], "int8")
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """2^32 + 4 is not 4: columns of the table (never touched), and numbers that are arguments."""
+    L, out = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    runs, n = torch.zeros(4, 8, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    table = torch.zeros(1, 4, dtype=torch.int32, device=DEV)
+    for at, v in ((6, 8 + (1 << 32)), (6, 8 - (1 << 32)), (7, 16 + (1 << 32)), (8, 1 + (1 << 32)), (8, 1 - (1 << 32))):
+        args = [table, L, L, out, runs, n, 8, 16, 1]
+        args[at] = v
+        with pytest.raises(RuntimeError, match="out of range"):
+            ops.kv_plan(*args)
+    wide = torch.empty(1, (1 << 32) + 4, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.kv_plan(wide, L, L, out, runs, n, 8, 16, 1)
+    c = R.Cache(1, 2, 1, 64, 16, "int8")
+    q = torch.zeros(1, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.attn_decode_paged(q.clone(), q, *c.parts(DEV), wide, L, "int8")
